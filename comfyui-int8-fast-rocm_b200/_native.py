@@ -21,6 +21,7 @@ ROT_NONE, ROT_REGULAR, ROT_SYLVESTER = range(3)
 WSCALE_TENSOR, WSCALE_ROW = 0, 1
 ROUND_NEAREST, ROUND_STOCHASTIC = 0, 1
 NORM_NONE, NORM_LAYER, NORM_RMS = range(3)
+ROUTE_SOFTMAX, ROUTE_SIGMOID = range(2)
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -63,6 +64,11 @@ SIGNATURES = {
     "qlin_dequant_asym_w4a8": [_P, _P, _P, _P, _I, _L, _L, _P, _P],
     "qlin_dequant_int8": [_P, _P, _I, _L, _L, _I, _I, _F, _P, _P],
     "qlin_requant_int8": [_P, _P, _I, _L, _L, _I, _I, _F, _I, _U64, _P, _P],
+    "qlin_route_experts_workspace": [_L, _L, _P],
+    "qlin_route_experts": [_P, _I, _L, _L, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "qlin_combine_experts": [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _L, _P, _P],
+    "qlin_gemm_w8a8_grouped": [_P, _P, _L, _P, _P, _P, _L, _P, _P, _P, _I, _L, _L, _L, _P],
+    "qlin_matvec_w4": [_P, _I, _L, _L, _P, _P, _I, _I, _P, _L, _P, _P, _P, _L, _L, _L, _P],
 }
 
 

@@ -654,4 +654,104 @@ QLIN_API int qlin_situ(const void* x, int x_dtype, int64_t M, int64_t K, int64_t
   return launch_situ(x_dtype, x, ldx, M, K, out, static_cast<cudaStream_t>(stream));
 }
 
+QLIN_API int qlin_route_experts_workspace(int64_t T, int64_t E, uint64_t* bytes) {
+  QLIN_RANGE();
+  if (!bytes) return fail(QLIN_ERR_INVALID_ARG, "bytes is null");
+  if (T < 0 || E < 1 || E > QLIN_MAX_EXPERTS) return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts");
+  *bytes = route_workspace_bytes(T, E);
+  return QLIN_OK;
+}
+
+QLIN_API int qlin_route_experts(const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t ld, int top_k,
+                                int scoring, int renormalize, int32_t* ids, float* weights, int32_t* offsets,
+                                int32_t* rows, int32_t* pos, void* workspace, uint64_t workspace_bytes,
+                                void* stream) {
+  QLIN_RANGE();
+  if (E < 1 || E > QLIN_MAX_EXPERTS) return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts");
+  if (T < 0 || ld < E) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  if (top_k < 1 || top_k > E || top_k > 32) return fail(QLIN_ERR_INVALID_ARG, "top_k must lie in 1 .. min(E, 32)");
+  if (!float_dt(logits_dtype)) return fail(QLIN_ERR_INVALID_ARG, "logits_dtype must be BF16, F16 or F32");
+  if (scoring != QLIN_ROUTE_SOFTMAX && scoring != QLIN_ROUTE_SIGMOID)
+    return fail(QLIN_ERR_INVALID_ARG, "bad scoring");
+  if (T > INT32_MAX / top_k) return fail(QLIN_ERR_UNSUPPORTED, "T * top_k must fit int32");
+  if (!offsets || (T > 0 && (!logits || !ids || !weights || !rows || !pos)))
+    return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  const uint64_t need = route_workspace_bytes(T, E);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(QLIN_ERR_INVALID_ARG, "workspace of " + std::to_string(need) + " bytes needed");
+  if (need && !aligned16(workspace)) return fail(QLIN_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  int rc = check_device();
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    const cudaError_t e = cudaMemsetAsync(offsets, 0, (size_t)(E + 1) * sizeof(int32_t), s);
+    return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "route offsets");
+  }
+  return launch_route(logits_dtype, logits, ld, T, E, top_k, scoring == QLIN_ROUTE_SIGMOID, renormalize != 0, ids,
+                      weights, offsets, rows, pos, workspace, s);
+}
+
+QLIN_API int qlin_combine_experts(const void* y, int dtype, int64_t R, int64_t N, int64_t ldy, const float* weights,
+                                  const int32_t* pos, int64_t T, int top_k, const void* residual, int64_t ld_res,
+                                  void* out, void* stream) {
+  QLIN_RANGE();
+  if (R < 0 || N < 0 || T < 0 || top_k < 1 || ldy < N || (residual && ld_res < N))
+    return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  if (!float_dt(dtype)) return fail(QLIN_ERR_INVALID_ARG, "dtype must be BF16, F16 or F32");
+  if (T == 0 || N == 0) return QLIN_OK;
+  if ((R > 0 && !y) || !weights || !pos || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  int rc = check_device();
+  if (rc) return rc;
+  return launch_combine(dtype, y, R, N, ldy, weights, pos, T, top_k, residual, ld_res, out,
+                        static_cast<cudaStream_t>(stream));
+}
+
+QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w,
+                                    const float* w_scale, const int32_t* offsets, int64_t E, const int32_t* a_rows,
+                                    const void* bias, void* out, int out_dtype, int64_t R, int64_t N, int64_t K,
+                                    void* stream) {
+  QLIN_RANGE();
+  if (E < 1 || E > QLIN_MAX_EXPERTS) return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts");
+  if (Ra < 0 || R < 0 || N < 0 || K <= 0 || (!a_rows && R != Ra)) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  if (K % 16) return fail(QLIN_ERR_ALIGNMENT, "K must be a multiple of 16");
+  if (!float_dt(out_dtype)) return fail(QLIN_ERR_INVALID_ARG, "out_dtype must be BF16, F16 or F32");
+  if (K > 131056) return fail(QLIN_ERR_UNSUPPORTED, "K above 131056 overflows the int32 sum");
+  if (R > INT32_MAX - 256 || Ra > INT32_MAX - 256 || N > INT32_MAX - 256 || E * N > INT32_MAX - 256)
+    return fail(QLIN_ERR_UNSUPPORTED, "dimension too large");
+  if (R == 0 || N == 0) return QLIN_OK;
+  if ((Ra > 0 && (!a || !a_scale)) || !w || !w_scale || !offsets || !out)
+    return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  if (!aligned16(a) || !aligned16(w) || !aligned16(out))
+    return fail(QLIN_ERR_ALIGNMENT, "operands must be 16-byte aligned");
+  int rc = check_device();
+  if (rc) return rc;
+  return launch_grouped(a, a_scale, Ra, w, w_scale, offsets, E, a_rows, bias, out, out_dtype, R, N, K,
+                        static_cast<cudaStream_t>(stream));
+}
+
+QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,
+                            const void* w_scale, int scale_dtype, int group, const int32_t* offsets, int64_t E,
+                            const int32_t* x_rows, const void* bias, void* out, int64_t R, int64_t N, int64_t K,
+                            void* stream) {
+  QLIN_RANGE();
+  if (E < 1 || E > QLIN_MAX_EXPERTS || (!offsets && E != 1))
+    return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts, one without offsets");
+  if (Rx < 0 || R < 0 || N < 0 || K <= 0 || K % 2 || ldx < K || (!x_rows && R != Rx))
+    return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  if (!float_dt(x_dtype)) return fail(QLIN_ERR_INVALID_ARG, "x_dtype must be BF16, F16 or F32");
+  if (scale_dtype != QLIN_F32 && scale_dtype != QLIN_BF16)
+    return fail(QLIN_ERR_INVALID_ARG, "scale_dtype must be F32 or BF16");
+  if (group != 0 && group != 128) return fail(QLIN_ERR_UNSUPPORTED, "int4 group must be 0 (per row) or 128");
+  if (group == 128 && K % 128) return fail(QLIN_ERR_INVALID_ARG, "K must be a multiple of 128 for group-128 int4");
+  if (R > INT32_MAX - 256 || Rx > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 256)
+    return fail(QLIN_ERR_UNSUPPORTED, "dimension too large");
+  if (R == 0 || N == 0) return QLIN_OK;
+  if ((Rx > 0 && !x) || !w_packed || !w_scale || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  int rc = check_device();
+  if (rc) return rc;
+  return launch_matvec_w4(x_dtype, x, Rx, ldx, reinterpret_cast<const uint8_t*>(w_packed), w_scale,
+                          scale_dtype == QLIN_F32 ? DT_F32 : DT_BF16, group ? (int)(K / group) : 1, offsets, E, x_rows,
+                          bias, out, R, N, K, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -158,6 +158,20 @@ int launch_requant_asym_w4a8(const uint8_t* packed, const float* codebook, const
 
 int launch_situ(int dt, const void* x, int64_t ldx, int64_t M, int64_t K, void* y, cudaStream_t stream);
 
+// Mixture-of-experts operators (experts.cu, grouped.cu, matvec.cu).
+size_t route_workspace_bytes(int64_t T, int64_t E);
+int launch_route(int dt, const void* logits, int64_t ld, int64_t T, int64_t E, int top_k, int sigmoid, int renorm,
+                 int32_t* ids, float* weights, int32_t* offsets, int32_t* rows, int32_t* pos, void* workspace,
+                 cudaStream_t stream);
+int launch_combine(int dt, const void* y, int64_t R, int64_t N, int64_t ldy, const float* weights, const int32_t* pos,
+                   int64_t T, int top_k, const void* residual, int64_t ld_res, void* out, cudaStream_t stream);
+int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
+                   const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
+                   int64_t R, int64_t N, int64_t K, cudaStream_t stream);
+int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
+                     int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
+                     int64_t R, int64_t N, int64_t K, cudaStream_t stream);
+
 int read_device_error(cudaStream_t stream, uint32_t* bits);
 // Failure detection: wait limits of the GEMM and row-kernel pipelines, the
 // one-thread wait self-tests, and a W8A8 GEMM whose producer leaves K-slab

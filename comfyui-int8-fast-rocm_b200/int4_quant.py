@@ -113,6 +113,20 @@ def convrot_w4a4_forward(x: Tensor, qweight: Tensor, wscales: Tensor, bias, conv
     return out.reshape(*orig_shape[:-1], wscales.shape[0])
 
 
+def convrot_w4a16_forward(x: Tensor, qweight: Tensor, wscales: Tensor, bias, convrot_groupsize: int,
+                          compute_dtype: torch.dtype, skip_rotation: bool = False) -> Tensor:
+    """:func:`convrot_w4a4_forward` for few rows (a modulation or embedding
+    linear, whose rows are the batch's samples) with the activation kept in
+    ``compute_dtype`` instead of quantised to int4; ``wscales`` [N], or
+    [N, K/128] for group-128 weights.  The weight is read at 4 bits, so such a
+    layer costs no more than the W4A4 one; no counterpart in the reference."""
+    if x.shape[-1] != qweight.shape[-1] * 2:
+        raise ValueError(f"Input K={x.shape[-1]} does not match packed qweight K={qweight.shape[-1] * 2}")
+    x_rot, orig_shape = prepare_rotated_activation(x, convrot_groupsize, compute_dtype, skip_rotation)
+    bias = None if bias is None else bias.to(device=x.device, dtype=compute_dtype)
+    return kops.matvec_w4(x_rot, qweight, wscales, bias).reshape(*orig_shape[:-1], qweight.shape[0])
+
+
 def quantize_signed_int4_packed_with_scale(x: Tensor, scale: Tensor) -> Tensor:
     """Packed int4 with a given per-row scale, ``round(x / s)`` clamped to
     +-7 (int4_quant.py:86-93); used when baking LoRA into an int4 layer."""

@@ -300,6 +300,60 @@ def _(w, scale, rot_kind, rot_group, stochastic, seed):
 
 
 # ---------------------------------------------------------------------------
+# (e) mixture-of-experts operators
+# ---------------------------------------------------------------------------
+
+
+@_op("route_experts")
+def _route_experts(logits: Tensor, top_k: int, scoring: str,
+                   renormalize: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return ops.route_experts(logits, top_k, scoring, renormalize)
+
+
+@_route_experts.register_fake
+def _(logits, top_k, scoring, renormalize):
+    T, E = _rows_of(logits), logits.shape[1]
+    i32 = dict(dtype=torch.int32)
+    return (logits.new_empty((T, top_k), **i32), logits.new_empty((T, top_k), dtype=torch.float32),
+            logits.new_empty((E + 1,), **i32), logits.new_empty((T * top_k,), **i32),
+            logits.new_empty((T, top_k), **i32))
+
+
+@_op("combine_experts")
+def _combine_experts(y: Tensor, weights: Tensor, pos: Tensor, residual: Optional[Tensor]) -> Tensor:
+    return ops.combine_experts(y, weights, pos, residual)
+
+
+@_combine_experts.register_fake
+def _(y, weights, pos, residual):
+    return y.new_empty((_rows_of(pos), y.shape[1]))
+
+
+@_op("gemm_w8a8_grouped")
+def _gemm_w8a8_grouped(a_q: Tensor, a_scale: Tensor, w_q: Tensor, w_scale: Tensor, offsets: Tensor,
+                       a_rows: Optional[Tensor], bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    return ops.gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows, bias, out_dtype)
+
+
+@_gemm_w8a8_grouped.register_fake
+def _(a_q, a_scale, w_q, w_scale, offsets, a_rows, bias, out_dtype):
+    R = _rows_of(a_q) if a_rows is None else a_rows.shape[0]
+    return a_q.new_empty((R, w_q.shape[1]), dtype=out_dtype)
+
+
+@_op("matvec_w4")
+def _matvec_w4(x: Tensor, w_packed: Tensor, w_scale: Tensor, bias: Optional[Tensor], offsets: Optional[Tensor],
+               x_rows: Optional[Tensor]) -> Tensor:
+    return ops.matvec_w4(x, w_packed, w_scale, bias, offsets, x_rows)
+
+
+@_matvec_w4.register_fake
+def _(x, w_packed, w_scale, bias, offsets, x_rows):
+    R = _rows_of(x) if x_rows is None else x_rows.shape[0]
+    return x.new_empty((R, w_packed.shape[-2]))
+
+
+# ---------------------------------------------------------------------------
 # callers' view: the signatures of ops.*, through the registered operators
 # ---------------------------------------------------------------------------
 
@@ -410,6 +464,22 @@ def dequant_int8(q: Tensor, scale, rot=None) -> Tensor:
 
 def requant_int8(w: Tensor, scale, rot=None, stochastic=False, seed=0) -> Tensor:
     return _L.requant_int8(w, _scale_tensor(scale, w.device), *_rot_args(rot), bool(stochastic), _signed64(seed))
+
+
+def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormalize: bool = True):
+    return _L.route_experts(logits, int(top_k), str(scoring), bool(renormalize))
+
+
+def combine_experts(y: Tensor, weights: Tensor, pos: Tensor, residual=None) -> Tensor:
+    return _L.combine_experts(y, weights, pos, residual)
+
+
+def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=None, out_dtype=torch.bfloat16):
+    return _L.gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows, bias, out_dtype)
+
+
+def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None) -> Tensor:
+    return _L.matvec_w4(x, w_packed, w_scale, bias, offsets, x_rows)
 
 
 hadamard_scale = ops.hadamard_scale

@@ -665,6 +665,217 @@ def requant_int8(w: torch.Tensor, scale, rot=None, stochastic=False, seed=0) -> 
     return q
 
 
+# ---------------------------------------------------------------------------
+# (e) mixture-of-experts operators
+# ---------------------------------------------------------------------------
+
+_SCORING = {"softmax": N.ROUTE_SOFTMAX, "sigmoid": N.ROUTE_SIGMOID}
+
+
+def _int32(t: torch.Tensor, numel, what: str, device) -> torch.Tensor:
+    """An index tensor as contiguous int32 on ``device``."""
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the other operands on {device}")
+    if t.dtype != torch.int32:
+        if t.dtype not in (torch.int64, torch.int16, torch.uint8, torch.int8):
+            raise TypeError(f"{what} must hold integers, got {t.dtype}")
+        t = t.to(torch.int32)
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{what} must have {numel} entries, got {t.numel()}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _vector(t: torch.Tensor, shape, what: str, dtype, device) -> torch.Tensor:
+    """A per-column (per-expert) parameter of ``shape`` (a trailing 1 is
+    dropped) as contiguous ``dtype`` on ``device``."""
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the other operands on {device}")
+    if tuple(t.shape) != shape and tuple(t.shape) != (*shape, 1):
+        raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", renormalize: bool = True):
+    """The ``top_k`` experts of every token and the plan that
+    :func:`gemm_w8a8_grouped`, :func:`matvec_w4` and :func:`combine_experts`
+    take.  ``logits`` [T, E] (bf16/f16/f32, row-strided views are read in
+    place), E <= 512, ``top_k`` <= min(E, 32).
+
+    Per token the largest logits in descending order, ties to the lowest
+    index; -inf (an expert switched off) and NaN are never chosen, and slots
+    that stay empty have id and position -1 and weight 0.  Weights, float32:
+    ``scoring`` "softmax" over all E logits or "sigmoid" of each, with
+    ``renormalize`` divided by their sum over the token's chosen experts.  A
+    NaN or +inf logit makes the token's softmax weights NaN.
+
+    Returns (ids int32 [T, k], weights float32 [T, k], offsets int32 [E + 1],
+    rows int32 [T * k], pos int32 [T, k]): sorted rows ``offsets[e] ..
+    offsets[e + 1]`` belong to expert e, ``rows`` holds their tokens (within
+    an expert in token order; -1 behind ``offsets[E]``) and ``pos`` the
+    sorted row of each (token, slot)."""
+    if logits.dim() != 2:
+        raise ValueError(f"expected [T, E] logits, got shape {tuple(logits.shape)}")
+    if scoring not in _SCORING:
+        raise ValueError(f"scoring must be one of {sorted(_SCORING)}, got {scoring!r}")
+    dt = dtype_code(logits.dtype)
+    T, E = logits.shape
+    top_k = int(top_k)
+    if not 1 <= E <= 512:
+        raise ValueError(f"between 1 and 512 experts, got {E}")
+    if not 1 <= top_k <= min(E, 32):
+        raise ValueError(f"top_k must lie between 1 and {min(E, 32)}, got {top_k}")
+    x, ld = _rows(logits)
+    st = _stream(x)
+    dev = x.device
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    offsets = torch.empty((E + 1,), dtype=torch.int32, device=dev)
+    rows = torch.empty((T * top_k,), dtype=torch.int32, device=dev)
+    pos = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    nbytes = ctypes.c_uint64(0)
+    N.call("qlin_route_experts_workspace", T, E, ctypes.addressof(nbytes))
+    ws = torch.empty((nbytes.value,), dtype=torch.uint8, device=dev) if nbytes.value else None
+    N.call("qlin_route_experts", x.data_ptr(), dt, T, E, max(ld, E), top_k, _SCORING[scoring], int(bool(renormalize)),
+           ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), pos.data_ptr(), _ptr(ws),
+           nbytes.value, st)
+    return ids, weights, offsets, rows, pos
+
+
+def combine_experts(y: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, residual=None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * y[pos[t, j]] (+ residual[t])``: the
+    experts' rows ``y`` [R, N] (bf16/f16/f32) back in token order, a float32
+    sum in slot order rounded once to y.dtype.  ``weights`` / ``pos`` [T, k]
+    as :func:`route_experts` returns them (a position outside [0, R), such as
+    -1, adds nothing), ``residual`` [T, N] in y.dtype."""
+    y, ldy = _rows(y)
+    R, Nn = y.shape
+    dt = dtype_code(y.dtype)
+    if pos.dim() != 2 or pos.shape[1] < 1 or tuple(weights.shape) != tuple(pos.shape):
+        raise ValueError(f"weights and pos must be [T, k], got {tuple(weights.shape)} and {tuple(pos.shape)}")
+    T, k = pos.shape
+    pos = _int32(pos, T * k, "pos", y.device)
+    weights = _vector(weights, (T, k), "weights", torch.float32, y.device)
+    ld_res = Nn
+    if residual is not None:
+        if tuple(residual.shape) != (T, Nn) or residual.dtype != y.dtype or residual.device != y.device:
+            raise ValueError(f"residual must be a [{T}, {Nn}] {y.dtype} tensor on {y.device}, got "
+                             f"{tuple(residual.shape)} {residual.dtype} on {residual.device}")
+        residual, ld_res = _rows(residual)
+    st = _stream(y)
+    out = torch.empty((T, Nn), dtype=y.dtype, device=y.device)
+    if T and Nn:
+        N.call("qlin_combine_experts", y.data_ptr(), dt, R, Nn, max(ldy, Nn), weights.data_ptr(), pos.data_ptr(), T,
+               k, _ptr(residual), max(ld_res, Nn), out.data_ptr(), st)
+    return out
+
+
+def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=None, out_dtype=torch.bfloat16):
+    """W8A8 linear of rows sorted by expert: rows ``offsets[e] ..
+    offsets[e + 1]`` of the result are :func:`gemm_w8a8` of those rows with
+    expert e's weight, bit for bit.  ``a_q`` [Ra, K] int8, ``a_scale`` [Ra]
+    (or [Ra, 1]), ``w_q`` [E, N, K] int8, ``w_scale`` [E, N], ``offsets``
+    int32 [E + 1] on the device, ``bias`` [E, N].
+
+    ``a_rows`` [R] gathers: result row r takes row ``a_rows[r]`` of ``a_q``
+    (the tokens' rows, quantised once; an index outside [0, Ra) is a row of
+    zeros).  Without it R = Ra.  Rows of no expert are 0.  The offsets stay
+    on the device: nothing synchronises, and any values are safe (clamped to
+    [0, R], each at least the one before)."""
+    if a_q.dtype != torch.int8 or w_q.dtype != torch.int8:
+        raise TypeError("int8 operands expected")
+    if a_q.dim() != 2 or w_q.dim() != 3:
+        raise ValueError(f"expected a [Ra, K] and an [E, N, K] operand, got {tuple(a_q.shape)} and {tuple(w_q.shape)}")
+    if a_q.shape[1] != w_q.shape[2]:
+        raise ValueError(f"K mismatch: activation K={a_q.shape[1]}, weight K={w_q.shape[2]}")
+    if a_q.device != w_q.device:
+        raise ValueError("operands on different devices")
+    dt = dtype_code(out_dtype)
+    dev = a_q.device
+    Ra = a_q.shape[0]
+    E, Nn, K = w_q.shape
+    if not 1 <= E <= 512:
+        raise ValueError(f"between 1 and 512 experts, got {E}")
+    offsets = _int32(offsets, E + 1, "offsets", dev)
+    a_scale = _vector(a_scale, (Ra,), "a_scale", torch.float32, dev)
+    w_scale = _vector(w_scale, (E, Nn), "w_scale", torch.float32, dev)
+    if a_rows is not None:
+        a_rows = _int32(a_rows, None, "a_rows", dev)
+        if a_rows.dim() != 1:
+            raise ValueError(f"a_rows must be one-dimensional, got shape {tuple(a_rows.shape)}")
+    if bias is not None:
+        bias = _vector(bias, (E, Nn), "bias", out_dtype, dev)
+    R = Ra if a_rows is None else a_rows.shape[0]
+    a_q, w_q = _pad_k(_aligned(a_q), _aligned(w_q), 16)
+    st = _stream(a_q)
+    out = torch.empty((R, Nn), dtype=out_dtype, device=dev)
+    if R and Nn:
+        N.call("qlin_gemm_w8a8_grouped", a_q.data_ptr(), a_scale.data_ptr(), Ra, w_q.data_ptr(), w_scale.data_ptr(),
+               offsets.data_ptr(), E, _ptr(a_rows), _ptr(bias), out.data_ptr(), dt, R, Nn, a_q.shape[1], st)
+    return out
+
+
+def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
+    """Linear of few rows with packed 4-bit weights, the activations kept in
+    their dtype: ``y = dt(x @ (q * scale).T + bias)`` with float32 sums and
+    one rounding.  ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in
+    place), ``w_packed`` [N, K/2] and ``w_scale`` [N] (or [N, 1]) or
+    [N, K/128], float32 or bfloat16, as :func:`quant_weight_int4` returns
+    them; ``bias`` [N]; the result is in x.dtype.
+
+    With ``offsets`` (int32 [E + 1] on the device) the rows are sorted by
+    expert: ``w_packed`` [E, N, K/2], ``w_scale`` [E, N] or [E, N, K/128],
+    ``bias`` [E, N]; rows of no expert are 0, and any offsets are safe (see
+    :func:`gemm_w8a8_grouped`).  ``x_rows`` [R] gathers: result row r takes
+    row ``x_rows[r]`` of ``x`` (an index outside [0, Rx) is a row of zeros).
+
+    The weights are read once for each 32 rows of an expert; many rows are
+    :func:`gemm_w4_g128`'s and :func:`gemm_w8a8_grouped`'s work."""
+    if w_packed.dtype != torch.int8:
+        raise TypeError("packed int4 weights are int8 tensors")
+    if x.device != w_packed.device:
+        raise ValueError("operands on different devices")
+    lead = 1 if offsets is None else 2
+    if w_packed.dim() != 1 + lead:
+        raise ValueError(f"expected {'an [E, N, K/2]' if lead == 2 else 'a [N, K/2]'} weight, got "
+                         f"{tuple(w_packed.shape)}")
+    dt = dtype_code(x.dtype)
+    dev = x.device
+    x, ldx = _rows(x)
+    Rx, K = x.shape
+    Nn, E = w_packed.shape[-2], (w_packed.shape[0] if lead == 2 else 1)
+    if K != 2 * w_packed.shape[-1]:
+        raise ValueError(f"K mismatch: activation K={K}, weight represents {2 * w_packed.shape[-1]}")
+    if not 1 <= E <= 512:
+        raise ValueError(f"between 1 and 512 experts, got {E}")
+    shape = tuple(w_packed.shape[:-1])
+    groups = w_scale.dim() == lead + 1 and w_scale.shape[-1] != 1
+    if groups and (K % 128 or w_scale.shape[-1] != K // 128):
+        raise ValueError(f"w_scale must be {list(shape)} or {[*shape, K // 128]} (128 k a group), got "
+                         f"{list(w_scale.shape)}")
+    w_scale = _vector(w_scale, (*shape, K // 128) if groups else shape, "w_scale",
+                      w_scale.dtype if w_scale.dtype == torch.bfloat16 else torch.float32, dev)
+    if offsets is not None:
+        offsets = _int32(offsets, E + 1, "offsets", dev)
+    if x_rows is not None:
+        x_rows = _int32(x_rows, None, "x_rows", dev)
+        if x_rows.dim() != 1:
+            raise ValueError(f"x_rows must be one-dimensional, got shape {tuple(x_rows.shape)}")
+    if bias is not None:
+        bias = _vector(bias, shape, "bias", x.dtype, dev)
+    if not w_packed.is_contiguous():
+        w_packed = w_packed.contiguous()
+    R = Rx if x_rows is None else x_rows.shape[0]
+    st = _stream(x)
+    out = torch.empty((R, Nn), dtype=x.dtype, device=dev)
+    if R and Nn:
+        N.call("qlin_matvec_w4", x.data_ptr(), dt, Rx, max(ldx, K), w_packed.data_ptr(), w_scale.data_ptr(),
+               dtype_code(w_scale.dtype), 128 if groups else 0, _ptr(offsets), E, _ptr(x_rows), _ptr(bias),
+               out.data_ptr(), R, Nn, K, st)
+    return out
+
+
 def device_error(device=None) -> int:
     """Read and clear the device-side error word (bit 0: a GEMM pipeline
     wait timed out; bit 1: a row-kernel wait timed out; bit 2: a timed-out

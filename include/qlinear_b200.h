@@ -413,6 +413,74 @@ QLIN_API int qlin_requant_int8(const float* w, const float* scale, int scale_mod
                                int rot_kind, int rot_group, float rot_c, int round_mode, uint64_t seed,
                                int8_t* q, void* stream);
 
+/* ---- (e) mixture-of-experts operators ------------------------------------
+ * No counterpart in the reference, whose linears are dense.  The router makes
+ * the plan that the products read:
+ *   offsets [E + 1]  rows [offsets[e], offsets[e + 1]) belong to expert e;
+ *   rows    [R]      the token (source row) of each sorted row;
+ *   pos     [T, k]   the sorted row of each (token, slot), -1 for none.
+ * The products take offsets as they come: values outside [0, R] are clamped
+ * and a value below an earlier one counts as that one, so no offsets make
+ * them leave their buffers. */
+
+#define QLIN_MAX_EXPERTS 512
+
+#define QLIN_ROUTE_SOFTMAX 0
+#define QLIN_ROUTE_SIGMOID 1
+
+/* logits [T, E] (row stride ld, BF16/F16/F32), 1 <= E <= QLIN_MAX_EXPERTS,
+ * 1 <= top_k <= min(E, 32), T * top_k < 2^31.  Per token the top_k largest logits in
+ * descending order, ties to the lowest index; -inf and NaN are never chosen,
+ * and the slots that stay empty get ids = pos = -1 and weight 0.
+ * weights (float32): softmax over all E logits, or the logits' sigmoids, in
+ * float32; with renormalize divided by their sum over the token's chosen
+ * experts.  A NaN or +inf among the logits makes the softmax weights NaN.
+ * offsets [E + 1], rows [T * top_k], pos [T, top_k]: the chosen pairs sorted
+ * by expert, within an expert by token; rows behind offsets[E] are -1.
+ * workspace: qlin_route_experts_workspace bytes of device memory, 16-byte
+ * aligned, used within the call only (NULL when that is 0). */
+QLIN_API int qlin_route_experts_workspace(int64_t T, int64_t E, uint64_t* bytes);
+QLIN_API int qlin_route_experts(const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t ld, int top_k,
+                                int scoring, int renormalize, int32_t* ids, float* weights, int32_t* offsets,
+                                int32_t* rows, int32_t* pos, void* workspace, uint64_t workspace_bytes,
+                                void* stream);
+
+/* out[t, n] = dt(sum_j weights[t, j] * y[pos[t, j], n] (+ residual[t, n])),
+ * a float32 sum in slot order (multiply-adds) and one rounding; slots whose
+ * pos lies outside [0, R) add nothing.  y [R, N] (row stride ldy), residual
+ * [T, N] (row stride ld_res, may be NULL) and out [T, N] share the dtype. */
+QLIN_API int qlin_combine_experts(const void* y, int dtype, int64_t R, int64_t N, int64_t ldy, const float* weights,
+                                  const int32_t* pos, int64_t T, int top_k, const void* residual, int64_t ld_res,
+                                  void* out, void* stream);
+
+/* W8A8 linear of rows sorted by expert: for the rows r of expert e,
+ *   out[r] = qlin_gemm_w8a8(a[src(r)], a_scale[src(r)], w[e], w_scale[e], bias[e])
+ * bit for bit (QLIN_WSCALE_ROW), src(r) = a_rows ? a_rows[r] : r.  a [Ra, K],
+ * w [E, N, K], w_scale [E, N], bias [E, N] in out_dtype or NULL, out [R, N];
+ * R = Ra without a_rows.  Rows of no expert become 0; a source row outside
+ * [0, Ra) counts as a row of zeros.  K % 16 == 0, K <= 131056 (the int32 sum
+ * holds any codes), 16-byte aligned operands. */
+QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w,
+                                    const float* w_scale, const int32_t* offsets, int64_t E, const int32_t* a_rows,
+                                    const void* bias, void* out, int out_dtype, int64_t R, int64_t N, int64_t K,
+                                    void* stream);
+
+/* Few rows times packed 4-bit weights, the activations kept in their dtype:
+ *   out[r, n] = dt(sum_g w_scale[n, g] * (sum_{k in g} x[src(r), k] * q[n, k]) + bias[n])
+ * with float32 sums and one rounding; q signed nibbles [N, K/2] (low nibble =
+ * even k), group 128 (K % 128 == 0) or 0 (one scale a row, any even K), the
+ * layouts of qlin_quant_weight_int4; w_scale F32 or BF16.  x [Rx, K] (row
+ * stride ldx) and bias [N] in x_dtype, out [R, N] in x_dtype.
+ * offsets NULL: E == 1, all rows use the one weight.  Otherwise w_packed
+ * [E, N, K/2], w_scale [E, N, G] and bias [E, N], rows sorted by expert; rows
+ * of no expert become 0.  src(r) = x_rows ? x_rows[r] : r; a source row
+ * outside [0, Rx) counts as a row of zeros.  Any R works; the weights are read
+ * once for each 32 rows of an expert, so many rows belong to the GEMMs. */
+QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,
+                            const void* w_scale, int scale_dtype, int group, const int32_t* offsets, int64_t E,
+                            const int32_t* x_rows, const void* bias, void* out, int64_t R, int64_t N, int64_t K,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif
