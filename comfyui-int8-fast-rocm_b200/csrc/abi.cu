@@ -145,10 +145,11 @@ QLIN_API int qlin_device_error(void* stream, uint32_t* error_bits) {
   if (!error_bits) return fail(QLIN_ERR_INVALID_ARG, "error_bits is null");
   int rc = check_device();
   if (rc) return rc;
-  uint32_t gemm_bits = 0, row_bits = 0;
+  uint32_t gemm_bits = 0, row_bits = 0, grouped_bits = 0;
   if ((rc = read_device_error(static_cast<cudaStream_t>(stream), &gemm_bits))) return rc;
   if ((rc = read_rowquant_error(static_cast<cudaStream_t>(stream), &row_bits))) return rc;
-  *error_bits = gemm_bits | row_bits;
+  if ((rc = read_grouped_error(static_cast<cudaStream_t>(stream), &grouped_bits))) return rc;
+  *error_bits = gemm_bits | row_bits | grouped_bits;
   return QLIN_OK;
 }
 
@@ -160,6 +161,7 @@ QLIN_API int qlin_set_wait_limit(uint64_t limit_ns) {
   if (limit_ns < 1000ull || limit_ns > 60000000000ull)
     return fail(QLIN_ERR_INVALID_ARG, "wait limit must lie between 1 us and 60 s");
   if ((rc = set_gemm_wait_limit(limit_ns))) return rc;
+  if ((rc = set_grouped_wait_limit(limit_ns))) return rc;
   return set_rowquant_wait_limit(limit_ns);
 }
 

@@ -274,6 +274,11 @@ void set_post(GemmParams& p, const EpiPost& e) {
 
 }  // namespace
 
+int encode_rows_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
+                     uint32_t box_rows) {
+  return make_tmap(m, base, row_bytes, rows, row_bytes, box_bytes, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 int launch_gemm(int kind, bool b_int4, const int8_t* a, const int8_t* b, const float* a_scale,
                 const float* w_scale, const void* bias, void* out, int out_dt, int64_t M, int64_t N, int64_t K,
                 cudaStream_t stream) {

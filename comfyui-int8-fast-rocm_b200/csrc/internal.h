@@ -1,6 +1,7 @@
 // Host-side declarations shared by the translation units of libqlinear_b200.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -158,6 +159,11 @@ int launch_requant_asym_w4a8(const uint8_t* packed, const float* codebook, const
 
 int launch_situ(int dt, const void* x, int64_t ldx, int64_t M, int64_t K, void* y, cudaStream_t stream);
 
+// Tensor map of `rows` contiguous rows of `row_bytes` bytes, boxes of
+// box_bytes x box_rows in the 128-byte swizzle (gemm.cu).
+int encode_rows_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
+                     uint32_t box_rows);
+
 // Mixture-of-experts operators (experts.cu, grouped.cu, matvec.cu).
 size_t route_workspace_bytes(int64_t T, int64_t E);
 int launch_route(int dt, const void* logits, int64_t ld, int64_t T, int64_t E, int top_k, int sigmoid, int renorm,
@@ -168,6 +174,8 @@ int launch_combine(int dt, const void* y, int64_t R, int64_t N, int64_t ldy, con
 int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
                    const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
                    int64_t R, int64_t N, int64_t K, cudaStream_t stream);
+int set_grouped_wait_limit(uint64_t ns);
+int read_grouped_error(cudaStream_t stream, uint32_t* bits);
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
                      int64_t R, int64_t N, int64_t K, cudaStream_t stream);
