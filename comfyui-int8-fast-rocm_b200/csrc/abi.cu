@@ -708,10 +708,18 @@ QLIN_API int qlin_combine_experts(const void* y, int dtype, int64_t R, int64_t N
                         static_cast<cudaStream_t>(stream));
 }
 
+QLIN_API int qlin_gemm_w8a8_grouped_workspace(int64_t R, int64_t K, uint64_t* bytes) {
+  QLIN_RANGE();
+  if (!bytes) return fail(QLIN_ERR_INVALID_ARG, "bytes is null");
+  if (R < 0 || K < 0 || R > INT32_MAX || K > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  *bytes = R == 0 ? 0 : grouped_workspace_bytes(R, K);
+  return QLIN_OK;
+}
+
 QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w,
                                     const float* w_scale, const int32_t* offsets, int64_t E, const int32_t* a_rows,
                                     const void* bias, void* out, int out_dtype, int64_t R, int64_t N, int64_t K,
-                                    void* stream) {
+                                    void* workspace, uint64_t workspace_bytes, void* stream) {
   QLIN_RANGE();
   if (E < 1 || E > QLIN_MAX_EXPERTS) return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts");
   if (Ra < 0 || R < 0 || N < 0 || K <= 0 || (!a_rows && R != Ra)) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
@@ -723,12 +731,15 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
   if (R == 0 || N == 0) return QLIN_OK;
   if ((Ra > 0 && (!a || !a_scale)) || !w || !w_scale || !offsets || !out)
     return fail(QLIN_ERR_INVALID_ARG, "null pointer");
-  if (!aligned16(a) || !aligned16(w) || !aligned16(out))
+  if (!aligned16(a) || !aligned16(w) || !aligned16(out) || (a_rows && !aligned16(workspace)))
     return fail(QLIN_ERR_ALIGNMENT, "operands must be 16-byte aligned");
+  if (a_rows && (!workspace || workspace_bytes < grouped_workspace_bytes(R, K)))
+    return fail(QLIN_ERR_INVALID_ARG,
+                "gathered rows need a workspace of " + std::to_string(grouped_workspace_bytes(R, K)) + " bytes");
   int rc = check_device();
   if (rc) return rc;
   return launch_grouped(a, a_scale, Ra, w, w_scale, offsets, E, a_rows, bias, out, out_dtype, R, N, K,
-                        static_cast<cudaStream_t>(stream));
+                        workspace, static_cast<cudaStream_t>(stream));
 }
 
 QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,

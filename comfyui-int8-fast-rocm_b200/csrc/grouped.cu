@@ -14,10 +14,16 @@
 // of up to 255 rows.
 //
 //   warp 0      producer: 128 bytes of K a stage of this CTA's 128 weight rows
-//               and of its half of the tile's rows, by TMA into a 6-stage
-//               ring; gathered rows by tile::gather4, four a lane
+//               and of its half of the tile's rows, one TMA box each, into a
+//               6-stage ring
 //   warp 1      TMEM and the pair's MMA issuer (leader CTA)
 //   warps 2-9   epilogue: lane = weight row, column = row of the expert
+//
+// Gathered rows are copied into their order first (gather_kernel): a TMA
+// instruction costs the producer about the same whatever it moves, and at 9
+// or 33 of them a stage (16-row boxes, tile::gather4) they bound the kernel:
+// 8192 rows, 8 experts, N 12288, K 4096: 341 us with boxes of 64 and 16 rows,
+// 432 us with 16, 927 us with gather4, the copy costs 14.
 //
 // Every wait is bounded; on a timeout the kernel sets the error word, waits
 // for its copies in flight, releases TMEM and returns.
@@ -64,7 +70,7 @@ __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
 constexpr int BM = 128;         // weight rows a CTA, 256 a pair
 constexpr int BK = 128;         // bytes of K a stage
 constexpr int BT = 256;         // rows of an expert a tile at most
-constexpr int BOX = 16;         // rows a TMA box of the activations
+constexpr int BOXES = 4;        // the activations' TMA boxes: 16, 32, 64 and 128 rows
 constexpr int STAGES = 6;
 constexpr int SLAB = BM * BK;   // 16 KB: a stage of either operand in one CTA
 constexpr int EPI_WARPS = 8;
@@ -73,12 +79,10 @@ constexpr int MAX_EXPERTS = QLIN_MAX_EXPERTS;
 constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
 
 struct GroupedParams {
-  const float* a_scale;    // [Ra]
-  int Ra;                  // rows of a; gathered indices outside read the tensor map's fill value, 0
+  const float* a_scale;    // [R]
   const float* w_scale;    // [E, N]
   const int32_t* offsets;  // [E + 1]
   int E;
-  const int32_t* a_rows;   // [R] or null
   const void* bias;        // [E, N] in the output dtype, or null
   void* out;               // [R, N]
   int R, N, K;
@@ -115,17 +119,6 @@ __device__ __forceinline__ Tile locate(const Smem* s, int tile, int& e) {
   t.rows = min(step, m - r);
   t.width = (t.rows + 31) & ~31;  // columns of the MMA
   return t;
-}
-
-// Four rows of the activations, chosen one by one, behind each other in
-// shared memory (a 128-byte slab each); counted on the pair leader's barrier.
-__device__ __forceinline__ void tma_gather4_pair(void* dst, const void* tmap, uint32_t mbar_cluster_addr, int x, int r0,
-                                                 int r1, int r2, int r3) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
-      "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(tmap), "r"(mbar_cluster_addr), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
-      : "memory");
 }
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
@@ -189,9 +182,13 @@ __device__ __forceinline__ void store_chunk(const GroupedParams& p, const uint32
   }
 }
 
-template <int DT, bool GATHER>
+struct RowMaps {
+  CUtensorMap box[BOXES];  // the activations in boxes of 16 << i rows
+};
+
+template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, GroupedParams p) {
+    grouped_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ RowMaps tmX, GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sW = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = sW + STAGES * SLAB;
@@ -265,51 +262,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     // ---------------- producer (both CTAs) ----------------
     if (lane == 0) {
       tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmX);
-    }
-    int stage = 0, e = 0;
-    uint32_t phase = 0, armed = 0, parity = 0;  // of the stages filled so far
-    bool ok = true;
-    for (int tile = first; tile < num_tiles && ok; tile += step) {
-      const Tile t = locate(s, tile, e);
-      const int half = t.width >> 1, mine = (int)rank * half;
-      const int wrow = t.e * p.N + t.n0 + (int)rank * BM;
-      int idx[4];
-      if constexpr (GATHER) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = mine + 4 * lane + i;
-          idx[i] = r < t.rows && 4 * lane < half ? p.a_rows[t.row0 + r] : -1;
-          if (idx[i] < 0 || idx[i] >= p.Ra) idx[i] = max(p.Ra, 1);  // behind the tensor map's rows: zeros
-        }
-      }
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (lane == 0) ok = wait_bounded(&s->empty[stage], phase ^ 1, abort_flag);
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        if (!ok) break;
-        const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
-        uint8_t* dx = sX + stage * SLAB;
-        if (lane == 0) {
-          if (leader) mbar_arrive_expect_tx(&s->full[stage], 2 * SLAB + t.width * BK);
+      for (int i = 0; i < BOXES; ++i) tma_prefetch_desc(&tmX.box[i]);
+      int stage = 0, e = 0;
+      uint32_t phase = 0, armed = 0, parity = 0;  // of the stages filled so far
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        const Tile t = locate(s, tile, e);
+        const int half = t.width >> 1;
+        const int wrow = t.e * p.N + t.n0 + (int)rank * BM, xrow = t.row0 + (int)rank * half;
+        // the smallest box that holds this CTA's rows (the MMA reads no more of them)
+        int box = 0;
+        while ((16 << box) < half) ++box;
+        const CUtensorMap* tmx = &tmX.box[box];
+        const uint32_t bytes = 2 * (SLAB + (16 << box) * BK);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
+          if (leader) mbar_arrive_expect_tx(&s->full[stage], bytes);
           tma_load_2d_pair(sW + stage * SLAB, &tmW, fb, kb * BK, wrow);
-          if constexpr (!GATHER) {
-            for (int b = 0; b < half; b += BOX) tma_load_2d_pair(dx + b * BK, &tmX, fb, kb * BK, t.row0 + mine + b);
-          }
+          tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
+          armed |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        if constexpr (GATHER) {
-          __syncwarp();
-          if (4 * lane < half) tma_gather4_pair(dx + 4 * lane * BK, &tmX, fb, kb * BK, idx[0], idx[1], idx[2], idx[3]);
-        }
-        armed |= 1u << stage;
-        parity = (parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
+      // no load still writing shared memory at exit (both CTAs' loads are
+      // counted by the leader; the peer waits for it at the last cluster barrier)
+      if (leader)
+        for (int i = 0; i < STAGES; ++i)
+          if (armed >> i & 1u) wait_drain(&s->full[i], parity >> i & 1u);
     }
-    // no load still writing shared memory at exit (both CTAs' loads are
-    // counted by the leader; the peer waits for it at the last cluster barrier)
-    if (leader && lane == 0)
-      for (int i = 0; i < STAGES; ++i)
-        if (armed >> i & 1u) wait_drain(&s->full[i], parity >> i & 1u);
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA) ----------------
     if (leader && lane == 0) {
@@ -367,11 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         ws = __ldg(p.w_scale + at);
         if (has_bias) bias = EO::to_f(reinterpret_cast<const typename EO::T*>(p.bias)[at]);
       }
-      if (tid < t.rows) {
-        int src = t.row0 + tid;
-        if constexpr (GATHER) src = p.a_rows[src];
-        if (src >= 0 && src < p.Ra) xs = __ldg(p.a_scale + src);
-      }
+      if (tid < t.rows) xs = __ldg(p.a_scale + t.row0 + tid);
       s->xs[acc][tid] = xs;
       wait_bounded(&s->tfull[acc], acc_phase, abort_flag);
       epilogue_barrier();
@@ -399,9 +377,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int DT, bool GATHER>
-int launch_dt(const CUtensorMap& tw, const CUtensorMap& tx, const GroupedParams& p, int clusters, cudaStream_t stream) {
-  auto kern = grouped_kernel<DT, GATHER>;
+// Rows a[rows[r]] and their scales in the order of r, zeros for an index
+// outside [0, Ra); a block takes `per` rows, a thread 16 bytes at a time.
+constexpr int GATHER_THREADS = 256;
+__global__ void __launch_bounds__(GATHER_THREADS)
+    gather_kernel(const int8_t* __restrict__ a, const float* __restrict__ a_scale, int64_t Ra,
+                  const int32_t* __restrict__ rows, int64_t R, int K16, int per, int8_t* __restrict__ out,
+                  float* __restrict__ out_scale) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t r0 = (int64_t)blockIdx.x * per;
+  const int count = (int)min((int64_t)per, R - r0);
+  const uint4* src = reinterpret_cast<const uint4*>(a);
+  uint4* dst = reinterpret_cast<uint4*>(out) + r0 * K16;
+  const int total = count * K16;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < total; i += GATHER_THREADS) {
+    const int64_t from = rows[r0 + i / K16];
+    dst[i] = from >= 0 && from < Ra ? src[from * K16 + i % K16] : make_uint4(0u, 0u, 0u, 0u);
+  }
+  for (int i = threadIdx.x; i < count; i += GATHER_THREADS) {
+    const int64_t from = rows[r0 + i];
+    out_scale[r0 + i] = from >= 0 && from < Ra ? a_scale[from] : 0.0f;
+  }
+}
+
+template <int DT>
+int launch_dt(const CUtensorMap& tw, const RowMaps& tx, const GroupedParams& p, int clusters, cudaStream_t stream) {
+  auto kern = grouped_kernel<DT>;
   static std::atomic<uint64_t> attr_devices{0};  // shared-memory limit raised once per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -416,29 +419,40 @@ int launch_dt(const CUtensorMap& tw, const CUtensorMap& tx, const GroupedParams&
   return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "grouped GEMM launch");
 }
 
+size_t gather_scale_offset(int64_t R, int64_t K) { return ((size_t)R * K + 15) & ~size_t(15); }
+
 }  // namespace
+
+size_t grouped_workspace_bytes(int64_t R, int64_t K) { return gather_scale_offset(R, K) + (size_t)R * sizeof(float); }
 
 int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
                    const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
-                   int64_t R, int64_t N, int64_t K, cudaStream_t stream) {
+                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream) {
   const int sms = device_sm_count();
   if (sms < 2) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
-  CUtensorMap tw, tx;
+  if (a_rows != nullptr) {
+    int8_t* sorted = static_cast<int8_t*>(workspace);
+    float* scale = reinterpret_cast<float*>(sorted + gather_scale_offset(R, K));
+    // about 16 KB a block: four 16-byte copies in flight a thread
+    const int per = (int)(K >= 16384 ? 1 : 16384 / K);
+    const cudaError_t e = launch_pdl(gather_kernel, dim3((unsigned)((R + per - 1) / per)), dim3(GATHER_THREADS), 0,
+                                     stream, a, a_scale, Ra, a_rows, R, (int)(K / 16), per, sorted, scale);
+    if (e != cudaSuccess) return cuda_fail(e, "grouped GEMM gather launch");
+    a = sorted;
+    a_scale = scale;
+  }
+  CUtensorMap tw;
+  RowMaps tx;
   int rc = encode_rows_tmap(&tw, w, (uint64_t)K, (uint64_t)(E * N), BK, BM);
+  for (int i = 0; i < BOXES && !rc; ++i) rc = encode_rows_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i);
   if (rc) return rc;
-  // (a without rows: any readable base; every gathered index lies behind it)
-  rc = encode_rows_tmap(&tx, Ra > 0 ? a : w, (uint64_t)K, (uint64_t)(Ra > 0 ? Ra : 1), BK, a_rows ? 1 : BOX);
-  if (rc) return rc;
-  const GroupedParams p{a_scale, (int)Ra, w_scale, offsets, (int)E, a_rows, bias, out, (int)R, (int)N, (int)K};
+  const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K};
   // tiles at most: every expert adds one partly filled row block to R / 256
   const int64_t tiles = (R / BT + (E < R ? E : R)) * ((N + 2 * BM - 1) / (2 * BM));
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);
-  const bool g = a_rows != nullptr;
-  if (out_dt == DT_BF16)
-    return g ? launch_dt<DT_BF16, true>(tw, tx, p, clusters, stream) : launch_dt<DT_BF16, false>(tw, tx, p, clusters, stream);
-  if (out_dt == DT_F16)
-    return g ? launch_dt<DT_F16, true>(tw, tx, p, clusters, stream) : launch_dt<DT_F16, false>(tw, tx, p, clusters, stream);
-  return g ? launch_dt<DT_F32, true>(tw, tx, p, clusters, stream) : launch_dt<DT_F32, false>(tw, tx, p, clusters, stream);
+  if (out_dt == DT_BF16) return launch_dt<DT_BF16>(tw, tx, p, clusters, stream);
+  if (out_dt == DT_F16) return launch_dt<DT_F16>(tw, tx, p, clusters, stream);
+  return launch_dt<DT_F32>(tw, tx, p, clusters, stream);
 }
 
 int set_grouped_wait_limit(uint64_t ns) {

@@ -811,8 +811,14 @@ def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=Non
     st = _stream(a_q)
     out = torch.empty((R, Nn), dtype=out_dtype, device=dev)
     if R and Nn:
+        K, ws, nbytes = a_q.shape[1], None, 0
+        if a_rows is not None:  # room for the rows in their order, freed (in stream order) with the call
+            need = ctypes.c_uint64(0)
+            N.call("qlin_gemm_w8a8_grouped_workspace", R, K, ctypes.addressof(need))
+            nbytes = need.value
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         N.call("qlin_gemm_w8a8_grouped", a_q.data_ptr(), a_scale.data_ptr(), Ra, w_q.data_ptr(), w_scale.data_ptr(),
-               offsets.data_ptr(), E, _ptr(a_rows), _ptr(bias), out.data_ptr(), dt, R, Nn, a_q.shape[1], st)
+               offsets.data_ptr(), E, _ptr(a_rows), _ptr(bias), out.data_ptr(), dt, R, Nn, K, _ptr(ws), nbytes, st)
     return out
 
 

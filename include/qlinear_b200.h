@@ -459,11 +459,15 @@ QLIN_API int qlin_combine_experts(const void* y, int dtype, int64_t R, int64_t N
  * w [E, N, K], w_scale [E, N], bias [E, N] in out_dtype or NULL, out [R, N];
  * R = Ra without a_rows.  Rows of no expert become 0; a source row outside
  * [0, Ra) counts as a row of zeros.  K % 16 == 0, K <= 131056 (the int32 sum
- * holds any codes), 16-byte aligned operands. */
+ * holds any codes), 16-byte aligned operands.
+ * With a_rows, workspace: qlin_gemm_w8a8_grouped_workspace(R, K) bytes of
+ * device memory, 16-byte aligned, used within the call only (the rows in
+ * their order); otherwise NULL. */
+QLIN_API int qlin_gemm_w8a8_grouped_workspace(int64_t R, int64_t K, uint64_t* bytes);
 QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w,
                                     const float* w_scale, const int32_t* offsets, int64_t E, const int32_t* a_rows,
                                     const void* bias, void* out, int out_dtype, int64_t R, int64_t N, int64_t K,
-                                    void* stream);
+                                    void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Few rows times packed 4-bit weights, the activations kept in their dtype:
  *   out[r, n] = dt(sum_g w_scale[n, g] * (sum_{k in g} x[src(r), k] * q[n, k]) + bias[n])

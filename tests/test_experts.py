@@ -804,12 +804,16 @@ def test_abi_refusals(pkg):
         y, dt, R, Nn, ld, 16, 16, T, k, res, ldr, 16, None)
     assert comb(ld=7) == comb(k=0) == comb(T=-1) == comb(res=16, ldr=7) == comb(dt=N.I8) == comb(y=None) == bad
     assert comb(T=0) == comb(Nn=0, ld=0) == 0
-    grp = lambda Ra=4, E=2, R=4, Nn=8, K=32, rows=None, off=16, dt=N.BF16, a=16, out=16: lib.qlin_gemm_w8a8_grouped(
-        a, 16, Ra, 16, 16, off, E, rows, None, out, dt, R, Nn, K, None)
+    grp = lambda Ra=4, E=2, R=4, Nn=8, K=32, rows=None, off=16, dt=N.BF16, a=16, out=16, ws=None, nws=0: lib.qlin_gemm_w8a8_grouped(
+        a, 16, Ra, 16, 16, off, E, rows, None, out, dt, R, Nn, K, ws, nws, None)
     assert grp(E=0) == grp(E=513) == grp(R=5) == grp(K=0) == grp(Nn=-1) == grp(off=None) == grp(dt=N.I8) == bad
     assert grp(K=20) == grp(a=24) == grp(out=20) == align
     assert grp(K=131072) == grp(E=512, Nn=2 ** 23) == unsup
     assert grp(R=0, Ra=0) == grp(Nn=0) == 0
+    assert lib.qlin_gemm_w8a8_grouped_workspace(4, 32, ctypes.addressof(n)) == 0 and n.value >= 4 * 32 + 4 * 4
+    assert lib.qlin_gemm_w8a8_grouped_workspace(-1, 32, ctypes.addressof(n)) == bad
+    assert grp(rows=16) == grp(rows=16, ws=16, nws=n.value - 16) == bad
+    assert grp(rows=16, ws=8, nws=4096) == align
     mv = lambda Rx=4, ld=256, sdt=N.F32, group=128, off=None, E=1, R=4, Nn=8, K=256, dt=N.BF16, x=16: lib.qlin_matvec_w4(
         x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, 16, R, Nn, K, None)
     assert mv(E=2) == mv(E=513, off=16) == mv(R=3) == mv(K=255) == mv(ld=255) == mv(sdt=N.F16) == mv(dt=N.I8) == bad
