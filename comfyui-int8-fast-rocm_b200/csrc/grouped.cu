@@ -17,7 +17,7 @@
 //               and of its half of the tile's rows, one TMA box each, into a
 //               6-stage ring
 //   warp 1      TMEM and the pair's MMA issuer (leader CTA)
-//   warps 2-9   epilogue: lane = weight row, column = row of the expert
+//   warps 2-17  epilogue: lane = weight row, column = row of the expert
 //
 // Gathered rows are copied into their order first (gather_kernel): a TMA
 // instruction costs the producer about the same whatever it moves, and at 9
@@ -71,9 +71,13 @@ constexpr int BM = 128;         // weight rows a CTA, 256 a pair
 constexpr int BK = 128;         // bytes of K a stage
 constexpr int BT = 256;         // rows of an expert a tile at most
 constexpr int BOXES = 4;        // the activations' TMA boxes: 16, 32, 64 and 128 rows
-constexpr int STAGES = 6;
+constexpr int MAX_STAGES = 6;
 constexpr int SLAB = BM * BK;   // 16 KB: a stage of either operand in one CTA
-constexpr int EPI_WARPS = 8;
+#ifndef EPIW
+#define EPIW 8
+#endif
+constexpr int EPI_WARPS = EPIW;     // four a quarter of the TMEM lanes: latencies overlap between them
+constexpr int CHUNK = 16;         // columns an epilogue warp takes at a time
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr int MAX_EXPERTS = QLIN_MAX_EXPERTS;
 constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns
@@ -89,14 +93,14 @@ struct GroupedParams {
 };
 
 struct Smem {  // behind the operand ring
-  uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], drain;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], drain;
   uint32_t tmem_slot;
   int abort_flag;
   alignas(16) float xs[2][BT];       // activation scales of a tile's rows
   int begin[MAX_EXPERTS + 1];        // first row of each expert, ascending within [0, R]
   int cum[MAX_EXPERTS + 1];          // tiles before each expert's
 };
-constexpr int SMEM_BYTES = 1024 + 2 * STAGES * SLAB + (int)sizeof(Smem);
+constexpr int SMEM_BYTES = 1024 + 2 * MAX_STAGES * SLAB + (int)sizeof(Smem);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 // A tile's place: expert, first weight row of the pair, first row and number
@@ -121,6 +125,13 @@ __device__ __forceinline__ Tile locate(const Smem* s, int tile, int& e) {
   return t;
 }
 
+// The smallest TMA box that holds a CTA's rows of the tile (the MMA reads no more of them).
+__device__ __forceinline__ int box_of(const Tile& t) {
+  int box = 0;
+  while ((32 << box) < t.width) ++box;
+  return box;
+}
+
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
 
 // Zeros in [b0, b1) bytes of the (16-byte aligned) output, both even, by `count` threads.
@@ -133,52 +144,85 @@ __device__ void zero_bytes(void* out, int64_t b0, int64_t b1, int64_t thread, in
   for (int64_t i = v1 + 2 * thread; i < b1; i += 2 * count) *reinterpret_cast<uint16_t*>(o + i) = 0;
 }
 
-// 32 columns (rows of the expert) of one accumulator: this thread has weight
-// row n of all of them.  16-bit results are exchanged between neighbouring
-// lanes so that each store writes two columns of one output row.
+// 32 lanes x 16 columns of 32-bit TMEM -> 16 registers, waited for.
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Two values rounded to the 16-bit dtype, the first in the low half.
 template <int DT>
-__device__ __forceinline__ void store_chunk(const GroupedParams& p, const uint32_t (&r)[32], const float* xs, float ws,
-                                            float bias, bool has_bias, int64_t row, int rows, int n, int lane) {
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == DT_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (DT == DT_F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+// CHUNK columns (rows of the expert) of one accumulator: this thread has
+// weight row n of all of them; out: element [first row, 0].  16-bit results
+// are exchanged between neighbouring lanes so that a store writes two columns
+// of one output row (a warp: two segments of 64 bytes).
+template <int DT>
+__device__ __forceinline__ void store_chunk(const uint32_t (&r)[CHUNK], const float* xs, float ws, float bias,
+                                            bool has_bias, typename Elem<DT>::T* out, int64_t N, int rows, int n,
+                                            int lane) {
   using EO = Elem<DT>;
-  using T = typename EO::T;
-  float y[32];
+  float y[CHUNK];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < CHUNK / 4; ++i) {
     const float4 x = reinterpret_cast<const float4*>(xs)[i];
     y[4 * i] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[4 * i]), x.x), ws);
     y[4 * i + 1] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[4 * i + 1]), x.y), ws);
     y[4 * i + 2] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[4 * i + 2]), x.z), ws);
     y[4 * i + 3] = __fmul_rn(__fmul_rn(__int2float_rn((int)r[4 * i + 3]), x.w), ws);
   }
-  if (has_bias) {
+  if constexpr (DT == DT_F32) {
+    if (n >= N) return;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(EO::round(y[j]), bias);
-  }
-  T* out = reinterpret_cast<T*>(p.out) + row * p.N;
-  if (DT == DT_F32 || (p.N & 1)) {
-    if (n < p.N) {
+    for (int j = 0; j < CHUNK; ++j)
+      if (j < rows) out[j * N + n] = has_bias ? __fadd_rn(y[j], bias) : y[j];
+  } else {
+    uint32_t w[CHUNK / 2];  // rows 2i and 2i + 1
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < rows) out[(int64_t)j * p.N + n] = EO::from_f(y[j]);
+    for (int i = 0; i < CHUNK / 2; ++i) {
+      w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
+      if (has_bias) {
+        const float2 v = unpack2<DT>(w[i]);
+        w[i] = pack2<DT>(__fadd_rn(v.x, bias), __fadd_rn(v.y, bias));
+      }
     }
-    return;
-  }
-  uint32_t* words = reinterpret_cast<uint32_t*>(out) + (n >> 1);
-  const int64_t pitch = p.N >> 1;
-  const int odd = lane & 1;
+    if (N & 1) {  // output rows off a word: one value a store
+      if (n >= N) return;
+      uint16_t* o = reinterpret_cast<uint16_t*>(out) + n;
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    uint32_t own;
-    if constexpr (DT == DT_F16) {
-      const __half2 h = __floats2half2_rn(y[j], y[j + 1]);
-      own = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(y[j], y[j + 1]);
-      own = *reinterpret_cast<const uint32_t*>(&h);
+      for (int j = 0; j < CHUNK; ++j)
+        if (j < rows) o[j * N] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+      return;
     }
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
-    const uint32_t w = odd ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
-    if (j + odd < rows && n < p.N) words[(j + odd) * pitch] = w;
+    const int odd = lane & 1;
+    uint32_t* o = reinterpret_cast<uint32_t*>(out) + odd * (N >> 1) + (n >> 1);
+#pragma unroll
+    for (int i = 0; i < CHUNK / 2; ++i) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], 1);
+      const uint32_t v = odd ? __byte_perm(other, w[i], 0x7632) : __byte_perm(w[i], other, 0x5410);
+      if (2 * i + odd < rows && n < N) *o = v;
+      o += N;
+    }
   }
 }
 
@@ -186,13 +230,16 @@ struct RowMaps {
   CUtensorMap box[BOXES];  // the activations in boxes of 16 << i rows
 };
 
-template <int DT>
+// SL slabs of 128 bytes of K a stage: 2 where rows are whole slabs (one TMA
+// box then covers both), else 1.
+template <int DT, int SL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ RowMaps tmX, GroupedParams p) {
+  constexpr int STAGES = MAX_STAGES / SL;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sW = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sX = sW + STAGES * SLAB;
-  Smem* s = reinterpret_cast<Smem*>(sX + STAGES * SLAB);
+  uint8_t* sX = sW + MAX_STAGES * SLAB;
+  Smem* s = reinterpret_cast<Smem*>(sX + MAX_STAGES * SLAB);
   volatile int* abort_flag = &s->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -255,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
   __syncthreads();
   const int num_tiles = s->cum[p.E];
-  const int num_kb = (p.K + BK - 1) / BK;
+  const int num_kb = (p.K + SL * BK - 1) / (SL * BK);
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
@@ -270,17 +317,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const Tile t = locate(s, tile, e);
         const int half = t.width >> 1;
         const int wrow = t.e * p.N + t.n0 + (int)rank * BM, xrow = t.row0 + (int)rank * half;
-        // the smallest box that holds this CTA's rows (the MMA reads no more of them)
-        int box = 0;
-        while ((16 << box) < half) ++box;
+        const int box = box_of(t);
         const CUtensorMap* tmx = &tmX.box[box];
-        const uint32_t bytes = 2 * (SLAB + (16 << box) * BK);
+        const uint32_t bytes = 2 * SL * (SLAB + (16 << box) * BK);
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
           const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
           if (leader) mbar_arrive_expect_tx(&s->full[stage], bytes);
-          tma_load_2d_pair(sW + stage * SLAB, &tmW, fb, kb * BK, wrow);
-          tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
+          if constexpr (SL == 1) {
+            tma_load_2d_pair(sW + stage * SLAB, &tmW, fb, kb * BK, wrow);
+            tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
+          } else {
+            tma_load_3d_pair(sW + stage * SL * SLAB, &tmW, fb, 0, wrow, kb * SL);
+            tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
+          }
           armed |= 1u << stage;
           parity = (parity & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -301,17 +351,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       for (int tile = first; tile < num_tiles && ok; tile += step) {
         const Tile t = locate(s, tile, e);
         const uint32_t idesc = umma_idesc_i8(2 * BM, t.width);
+        const uint32_t xslab = (16u << box_of(t)) * BK;  // from one slab of the rows to the next
         if (!wait_bounded(&s->tempty[acc], acc_phase ^ 1, abort_flag)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * BT;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!wait_bounded(&s->full[stage], phase, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t wdesc = umma_desc_k_sw128(smem_u32(sW + stage * SLAB));
-          const uint64_t xdesc = umma_desc_k_sw128(smem_u32(sX + stage * SLAB));
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_i8_pair(d, wdesc + 2 * k, xdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          for (int h = 0; h < SL; ++h) {
+            const uint64_t wdesc = umma_desc_k_sw128(smem_u32(sW + (stage * SL + h) * SLAB));
+            const uint64_t xdesc = umma_desc_k_sw128(smem_u32(sX + stage * SL * SLAB) + h * xslab);
+#pragma unroll
+            for (int k = 0; k < BK / 32; ++k)
+              umma_i8_pair(d, wdesc + 2 * k, xdesc + 2 * k, idesc, (kb | h | k) != 0 ? 1u : 0u);
+          }
           issued = true;
           umma_commit_pair(&s->empty[stage], 0x3);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -329,9 +383,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   } else {
     // ---------------- epilogue (both CTAs) ----------------
     using EO = Elem<DT>;
-    const int tid = threadIdx.x - 64, quarter = warp & 3, half = (warp - 2) >> 2;
+    using T = typename EO::T;
+    const int tid = threadIdx.x - 64, quarter = warp & 3, part = (warp - 2) >> 2;
     {  // rows of no expert
-      const int64_t line = (int64_t)p.N * sizeof(typename EO::T);
+      const int64_t line = (int64_t)p.N * sizeof(T);
       const int64_t thread = (int64_t)blockIdx.x * 32 * EPI_WARPS + tid, count = (int64_t)gridDim.x * 32 * EPI_WARPS;
       if (s->begin[0] > 0) zero_bytes(p.out, 0, s->begin[0] * line, thread, count);
       if (s->begin[p.E] < p.R) zero_bytes(p.out, s->begin[p.E] * line, p.R * line, thread, count);
@@ -339,27 +394,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     int acc = 0, e = 0;
     uint32_t acc_phase = 0;
     const bool has_bias = p.bias != nullptr;
-    for (int tile = first; tile < num_tiles; tile += step) {
-      const Tile t = locate(s, tile, e);
-      // this tile's scales and bias, while its products are computed
-      const int n = t.n0 + (int)rank * BM + quarter * 32 + lane;
-      float ws = 0.0f, bias = 0.0f, xs = 0.0f;
+    // a tile's scales and bias, read while the tile before it is converted
+    Tile t{};
+    int n = 0;
+    float ws = 0.0f, bias = 0.0f, xs = 0.0f;
+    auto fetch = [&](int tile) {
+      t = locate(s, tile, e);
+      n = t.n0 + (int)rank * BM + quarter * 32 + lane;
+      ws = bias = xs = 0.0f;
       if (n < p.N) {
         const int64_t at = (int64_t)t.e * p.N + n;
         ws = __ldg(p.w_scale + at);
-        if (has_bias) bias = EO::to_f(reinterpret_cast<const typename EO::T*>(p.bias)[at]);
+        if (has_bias) bias = EO::to_f(reinterpret_cast<const T*>(p.bias)[at]);
       }
       if (tid < t.rows) xs = __ldg(p.a_scale + t.row0 + tid);
-      s->xs[acc][tid] = xs;
-      wait_bounded(&s->tfull[acc], acc_phase, abort_flag);
+    };
+    if (first < num_tiles) fetch(first);
+    for (int tile = first; tile < num_tiles; tile += step) {
+      const Tile now = t;
+      const int col = n;
+      const float wscale = ws, b = bias;
+      if (tid < BT) s->xs[acc][tid] = xs;
+      // one thread polls; the others sleep at the barrier
+      if (tid == 0) wait_bounded(&s->tfull[acc], acc_phase, abort_flag);
       epilogue_barrier();
       if (*abort_flag) break;
       tc_fence_after();
-      for (int c = half * 32; c < t.rows; c += 64) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + acc * BT + c + ((uint32_t)(quarter * 32) << 16), r);
-        tmem_ld_wait_regs(r);
-        store_chunk<DT>(p, r, &s->xs[acc][c], ws, bias, has_bias, t.row0 + c, t.rows - c, n, lane);
+      if (tile + step < num_tiles) fetch(tile + step);
+      for (int c = part * CHUNK; c < now.rows; c += EPI_WARPS / 4 * CHUNK) {
+        uint32_t r[CHUNK];
+        tmem_ld_16(tmem_base + acc * BT + c + ((uint32_t)(quarter * 32) << 16), r);
+        store_chunk<DT>(r, &s->xs[acc][c], wscale, b, has_bias,
+                        reinterpret_cast<T*>(p.out) + (int64_t)(now.row0 + c) * p.N, p.N, now.rows - c, col, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -402,9 +468,9 @@ __global__ void __launch_bounds__(GATHER_THREADS)
   }
 }
 
-template <int DT>
+template <int DT, int SL>
 int launch_dt(const CUtensorMap& tw, const RowMaps& tx, const GroupedParams& p, int clusters, cudaStream_t stream) {
-  auto kern = grouped_kernel<DT>;
+  auto kern = grouped_kernel<DT, SL>;
   static std::atomic<uint64_t> attr_devices{0};  // shared-memory limit raised once per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -443,16 +509,21 @@ int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8
   }
   CUtensorMap tw;
   RowMaps tx;
-  int rc = encode_rows_tmap(&tw, w, (uint64_t)K, (uint64_t)(E * N), BK, BM);
-  for (int i = 0; i < BOXES && !rc; ++i) rc = encode_rows_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i);
+  const int slabs = K % BK == 0 ? 2 : 1;
+  int rc = encode_slab_tmap(&tw, w, (uint64_t)K, (uint64_t)(E * N), BK, BM, slabs);
+  for (int i = 0; i < BOXES && !rc; ++i)
+    rc = encode_slab_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i, slabs);
   if (rc) return rc;
   const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K};
   // tiles at most: every expert adds one partly filled row block to R / 256
   const int64_t tiles = (R / BT + (E < R ? E : R)) * ((N + 2 * BM - 1) / (2 * BM));
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);
-  if (out_dt == DT_BF16) return launch_dt<DT_BF16>(tw, tx, p, clusters, stream);
-  if (out_dt == DT_F16) return launch_dt<DT_F16>(tw, tx, p, clusters, stream);
-  return launch_dt<DT_F32>(tw, tx, p, clusters, stream);
+#define QLIN_GROUPED(DT)                                                                                   \
+  return slabs == 2 ? launch_dt<DT, 2>(tw, tx, p, clusters, stream) : launch_dt<DT, 1>(tw, tx, p, clusters, stream)
+  if (out_dt == DT_BF16) QLIN_GROUPED(DT_BF16);
+  if (out_dt == DT_F16) QLIN_GROUPED(DT_F16);
+  QLIN_GROUPED(DT_F32);
+#undef QLIN_GROUPED
 }
 
 int set_grouped_wait_limit(uint64_t ns) {

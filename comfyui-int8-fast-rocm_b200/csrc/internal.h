@@ -160,9 +160,11 @@ int launch_requant_asym_w4a8(const uint8_t* packed, const float* codebook, const
 int launch_situ(int dt, const void* x, int64_t ldx, int64_t M, int64_t K, void* y, cudaStream_t stream);
 
 // Tensor map of `rows` contiguous rows of `row_bytes` bytes, boxes of
-// box_bytes x box_rows in the 128-byte swizzle (gemm.cu).
-int encode_rows_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
-                     uint32_t box_rows);
+// slab_bytes x box_rows in the 128-byte swizzle; with slabs > 1 (row_bytes a
+// multiple of slab_bytes) three-dimensional, {byte in slab, row, slab}, and
+// boxes of that many slabs behind each other (gemm.cu).
+int encode_slab_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
+                     uint32_t box_rows, uint32_t slabs);
 
 // Mixture-of-experts operators (experts.cu, grouped.cu, matvec.cu).
 size_t route_workspace_bytes(int64_t T, int64_t E);
