@@ -145,11 +145,12 @@ QLIN_API int qlin_device_error(void* stream, uint32_t* error_bits) {
   if (!error_bits) return fail(QLIN_ERR_INVALID_ARG, "error_bits is null");
   int rc = check_device();
   if (rc) return rc;
-  uint32_t gemm_bits = 0, row_bits = 0, grouped_bits = 0;
+  uint32_t gemm_bits = 0, row_bits = 0, grouped_bits = 0, matvec_bits = 0;
   if ((rc = read_device_error(static_cast<cudaStream_t>(stream), &gemm_bits))) return rc;
   if ((rc = read_rowquant_error(static_cast<cudaStream_t>(stream), &row_bits))) return rc;
   if ((rc = read_grouped_error(static_cast<cudaStream_t>(stream), &grouped_bits))) return rc;
-  *error_bits = gemm_bits | row_bits | grouped_bits;
+  if ((rc = read_matvec_error(static_cast<cudaStream_t>(stream), &matvec_bits))) return rc;
+  *error_bits = gemm_bits | row_bits | grouped_bits | matvec_bits;
   return QLIN_OK;
 }
 
@@ -162,6 +163,7 @@ QLIN_API int qlin_set_wait_limit(uint64_t limit_ns) {
     return fail(QLIN_ERR_INVALID_ARG, "wait limit must lie between 1 us and 60 s");
   if ((rc = set_gemm_wait_limit(limit_ns))) return rc;
   if ((rc = set_grouped_wait_limit(limit_ns))) return rc;
+  if ((rc = set_matvec_wait_limit(limit_ns))) return rc;
   return set_rowquant_wait_limit(limit_ns);
 }
 
@@ -742,10 +744,18 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
                         workspace, static_cast<cudaStream_t>(stream));
 }
 
+QLIN_API int qlin_matvec_w4_workspace(int64_t Rx, int64_t K, uint64_t* bytes) {
+  QLIN_RANGE();
+  if (!bytes) return fail(QLIN_ERR_INVALID_ARG, "bytes is null");
+  if (Rx < 0 || K < 0 || Rx > INT32_MAX || K > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  *bytes = matvec_workspace_bytes(Rx, K);
+  return QLIN_OK;
+}
+
 QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,
                             const void* w_scale, int scale_dtype, int group, const int32_t* offsets, int64_t E,
                             const int32_t* x_rows, const void* bias, void* out, int64_t R, int64_t N, int64_t K,
-                            void* stream) {
+                            void* workspace, uint64_t workspace_bytes, void* stream) {
   QLIN_RANGE();
   if (E < 1 || E > QLIN_MAX_EXPERTS || (!offsets && E != 1))
     return fail(QLIN_ERR_INVALID_ARG, "between 1 and 512 experts, one without offsets");
@@ -760,11 +770,14 @@ QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx,
     return fail(QLIN_ERR_UNSUPPORTED, "dimension too large");
   if (R == 0 || N == 0) return QLIN_OK;
   if ((Rx > 0 && !x) || !w_packed || !w_scale || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  if (Rx > 0 && (!workspace || workspace_bytes < matvec_workspace_bytes(Rx, K)))
+    return fail(QLIN_ERR_INVALID_ARG, "workspace of " + std::to_string(matvec_workspace_bytes(Rx, K)) + " bytes needed");
+  if (!aligned16(workspace)) return fail(QLIN_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
   int rc = check_device();
   if (rc) return rc;
   return launch_matvec_w4(x_dtype, x, Rx, ldx, reinterpret_cast<const uint8_t*>(w_packed), w_scale,
                           scale_dtype == QLIN_F32 ? DT_F32 : DT_BF16, group ? (int)(K / group) : 1, offsets, E, x_rows,
-                          bias, out, R, N, K, static_cast<cudaStream_t>(stream));
+                          bias, out, R, N, K, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,4 +1,5 @@
 // Host side of the tcgen05 GEMMs: TMA descriptors, tile configuration, launch.
+#include <array>
 #include <atomic>
 #include <cstdint>
 #include <cstdlib>
@@ -65,6 +66,20 @@ int make_tmap3(CUtensorMap* m, const void* base, uint64_t inner, uint64_t seg_ro
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(QLIN_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed (code " + std::to_string((int)r) + ")");
+  return QLIN_OK;
+}
+
+// 3-D tensor map of bytes in the 128-byte swizzle.
+int make_tmap_slabs(CUtensorMap* m, const void* base, const std::array<cuuint64_t, 3>& dims,
+                    const std::array<cuuint64_t, 2>& strides, const std::array<cuuint32_t, 3>& box) {
+  PFN_encodeTiled_t enc = get_encode_fn();
+  if (!enc) return fail(QLIN_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims.data(), strides.data(), box.data(),
+                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(QLIN_ERR_CUDA, "cuTensorMapEncodeTiled (slabs) failed (code " + std::to_string((int)r) + ")");
   return QLIN_OK;
 }
 
@@ -277,18 +292,14 @@ void set_post(GemmParams& p, const EpiPost& e) {
 int encode_slab_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
                      uint32_t box_rows, uint32_t slabs) {
   if (slabs == 1) return make_tmap(m, base, row_bytes, rows, row_bytes, slab_bytes, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
-  PFN_encodeTiled_t enc = get_encode_fn();
-  if (!enc) return fail(QLIN_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
-  cuuint64_t dims[3] = {slab_bytes, rows, row_bytes / slab_bytes};
-  cuuint64_t strides[2] = {row_bytes, slab_bytes};
-  cuuint32_t box[3] = {slab_bytes, box_rows, slabs};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(QLIN_ERR_CUDA, "cuTensorMapEncodeTiled (slabs) failed (code " + std::to_string((int)r) + ")");
-  return QLIN_OK;
+  return make_tmap_slabs(m, base, {slab_bytes, rows, row_bytes / slab_bytes}, {row_bytes, slab_bytes},
+                         {slab_bytes, box_rows, slabs});
+}
+
+int encode_row_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
+                    uint32_t box_rows, uint32_t slabs) {
+  return make_tmap_slabs(m, base, {slab_bytes, row_bytes / slab_bytes, rows}, {slab_bytes, row_bytes},
+                         {slab_bytes, slabs, box_rows});
 }
 
 int launch_gemm(int kind, bool b_int4, const int8_t* a, const int8_t* b, const float* a_scale,

@@ -30,42 +30,10 @@
 #include <atomic>
 
 #include "../../include/qlinear_b200.h"
-#include "common.cuh"
-#include "internal.h"
+#include "bounded.cuh"
 
 namespace qlin {
 namespace {
-
-__device__ uint32_t g_grouped_error_bits = 0;             // as the dense GEMM's: 1 timed out, 4 not drained
-__device__ uint64_t g_grouped_wait_limit_ns = 2000000000ull;
-
-__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t limit = *reinterpret_cast<volatile uint64_t*>(&g_grouped_wait_limit_ns);
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t iter = 0;
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((++iter & 63u) == 0) {
-      if (*abort) return false;
-      if (globaltimer_ns() - t0 > limit) {
-        atomicOr(&g_grouped_error_bits, 1u);
-        *abort = 1;
-        return false;
-      }
-    }
-  }
-}
-__device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
-  const uint64_t limit = *reinterpret_cast<volatile uint64_t*>(&g_grouped_wait_limit_ns);
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > limit) {
-      atomicOr(&g_grouped_error_bits, 4u);
-      return;
-    }
-  }
-}
 
 constexpr int BM = 128;         // weight rows a CTA, 256 a pair
 constexpr int BK = 128;         // bytes of K a stage
@@ -133,16 +101,6 @@ __device__ __forceinline__ int box_of(const Tile& t) {
 }
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
-
-// Zeros in [b0, b1) bytes of the (16-byte aligned) output, both even, by `count` threads.
-__device__ void zero_bytes(void* out, int64_t b0, int64_t b1, int64_t thread, int64_t count) {
-  char* o = static_cast<char*>(out);
-  const int64_t v0 = min((b0 + 15) & ~int64_t(15), b1), v1 = max(b1 & ~int64_t(15), v0);
-  for (int64_t i = v0 + 16 * thread; i < v1; i += 16 * count)
-    *reinterpret_cast<uint4*>(o + i) = make_uint4(0u, 0u, 0u, 0u);
-  for (int64_t i = b0 + 2 * thread; i < v0; i += 2 * count) *reinterpret_cast<uint16_t*>(o + i) = 0;
-  for (int64_t i = v1 + 2 * thread; i < b1; i += 2 * count) *reinterpret_cast<uint16_t*>(o + i) = 0;
-}
 
 // 32 lanes x 16 columns of 32-bit TMEM -> 16 registers, waited for.
 __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -273,33 +231,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   for (int e = threadIdx.x; e <= p.E; e += THREADS) s->begin[e] = min(max(p.offsets[e], 0), p.R);
   __syncthreads();
   const int num_n = (p.N + 2 * BM - 1) / (2 * BM);
-  if (warp == 0) {
-    int top = 0, tiles = 0;
-    for (int e0 = 0; e0 <= p.E; e0 += 32) {
-      const int e = e0 + lane;
-      int b = e <= p.E ? s->begin[e] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, b, o);
-        if (lane >= o) b = max(b, u);
-      }
-      b = max(b, top);
-      int before = __shfl_up_sync(0xffffffffu, b, 1);
-      if (lane == 0) before = e0 == 0 ? b : top;
-      int n = e <= p.E ? (b - before + BT - 1) / BT * num_n : 0;  // tiles of expert e - 1
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += u;
-      }
-      if (e <= p.E) {
-        s->begin[e] = b;
-        s->cum[e] = tiles + n;
-      }
-      top = __shfl_sync(0xffffffffu, b, 31);
-      tiles += __shfl_sync(0xffffffffu, n, 31);
-    }
-  }
+  if (warp == 0)
+    expert_bounds(s->begin, s->cum, p.E, lane, [=](int rows) { return (rows + BT - 1) / BT * num_n; });
   __syncthreads();
   const int num_tiles = s->cum[p.E];
   const int num_kb = (p.K + SL * BK - 1) / (SL * BK);
@@ -311,7 +244,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       tma_prefetch_desc(&tmW);
       for (int i = 0; i < BOXES; ++i) tma_prefetch_desc(&tmX.box[i]);
       int stage = 0, e = 0;
-      uint32_t phase = 0, armed = 0, parity = 0;  // of the stages filled so far
+      uint32_t phase = 0;
+      Armed armed;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step) {
         const Tile t = locate(s, tile, e);
@@ -331,16 +265,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tma_load_3d_pair(sW + stage * SL * SLAB, &tmW, fb, 0, wrow, kb * SL);
             tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
           }
-          armed |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
+          armed.note(stage, phase);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
       // no load still writing shared memory at exit (both CTAs' loads are
       // counted by the leader; the peer waits for it at the last cluster barrier)
-      if (leader)
-        for (int i = 0; i < STAGES; ++i)
-          if (armed >> i & 1u) wait_drain(&s->full[i], parity >> i & 1u);
+      if (leader) armed.drain(s->full);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA) ----------------
@@ -526,23 +457,7 @@ int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8
 #undef QLIN_GROUPED
 }
 
-int set_grouped_wait_limit(uint64_t ns) {
-  const cudaError_t e = cudaMemcpyToSymbol(g_grouped_wait_limit_ns, &ns, sizeof(ns));
-  return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "set grouped GEMM wait limit");
-}
-
-int read_grouped_error(cudaStream_t stream, uint32_t* bits) {
-  uint32_t h = 0;
-  cudaError_t e =
-      cudaMemcpyFromSymbolAsync(&h, g_grouped_error_bits, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "read grouped GEMM error word");
-  const uint32_t zero = 0;
-  e = cudaMemcpyToSymbolAsync(g_grouped_error_bits, &zero, sizeof(uint32_t), 0, cudaMemcpyHostToDevice, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "clear grouped GEMM error word");
-  e = cudaStreamSynchronize(stream);
-  if (e != cudaSuccess) return cuda_fail(e, "sync");
-  *bits = h;
-  return QLIN_OK;
-}
+int set_grouped_wait_limit(uint64_t ns) { return set_tu_wait_limit(ns); }
+int read_grouped_error(cudaStream_t stream, uint32_t* bits) { return read_tu_error(stream, bits); }
 
 }  // namespace qlin

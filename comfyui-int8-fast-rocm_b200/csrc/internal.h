@@ -165,6 +165,10 @@ int launch_situ(int dt, const void* x, int64_t ldx, int64_t M, int64_t K, void* 
 // boxes of that many slabs behind each other (gemm.cu).
 int encode_slab_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
                      uint32_t box_rows, uint32_t slabs);
+// The same rows as {byte in slab, slab, row}: boxes of box_rows rows of
+// `slabs` slabs each, a row's slabs behind each other.
+int encode_row_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
+                    uint32_t box_rows, uint32_t slabs);
 
 // Mixture-of-experts operators (experts.cu, grouped.cu, matvec.cu).
 size_t route_workspace_bytes(int64_t T, int64_t E);
@@ -181,7 +185,10 @@ int set_grouped_wait_limit(uint64_t ns);
 int read_grouped_error(cudaStream_t stream, uint32_t* bits);
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
-                     int64_t R, int64_t N, int64_t K, cudaStream_t stream);
+                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream);
+size_t matvec_workspace_bytes(int64_t Rx, int64_t K);
+int set_matvec_wait_limit(uint64_t ns);
+int read_matvec_error(cudaStream_t stream, uint32_t* bits);
 
 int read_device_error(cudaStream_t stream, uint32_t* bits);
 // Failure detection: wait limits of the GEMM and row-kernel pipelines, the

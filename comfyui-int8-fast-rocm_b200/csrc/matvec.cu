@@ -4,95 +4,770 @@
 // Unlike the W4A8 / W4A4 GEMMs the activations are not quantised.  With
 // offsets [E + 1] the rows are sorted by expert and each uses its expert's
 // weights.
+//
+// The weights' bytes bound it if a nibble costs next to nothing: at the HBM
+// rate an SM receives 46 of them a clock.  As integers they cost 3/8 of an
+// instruction each (a mask puts four into the high halves of four bytes, 16 q,
+// without sign extension; as bf16 they take 11/8), so the activations become
+// integers too, without losing theirs:
+//
+//   split_kernel   each 128 k of a row (a weight scale's group) as 32-bit
+//                  integers X = x * 2^(29 - e), e the exponent of the largest
+//                  of them, each in four signed base-256 digits.  A value down
+//                  to 2^-6 (float32), 2^-19 (f16) or 2^-22 (bf16) of the
+//                  largest is exact, a smaller one off by 2^-30 of it at most,
+//                  less than a float32 sum of them loses;
+//   matvec_kernel  mma.sync m16n8k32 (int8): 16 weight rows times 8 columns,
+//                  the four digits of two rows.  The int32 sums of a block of
+//                  128 are exact; digits and scales meet once a block in
+//                  float32.
+//
+// matvec_kernel is persistent, a block of threads a SM.  One warp brings the
+// weights by TMA, 32 or 16 KB a stage of 32 rows or more (loads of 64 bytes a
+// row straight into the lanes that need them stayed at 2 TB/s).  One brings an
+// expert's activation digits, which stay in shared memory for all its row
+// tiles.  Eight warps multiply, each 32 rows and one or two blocks of 128 k of
+// a stage.  One adds their sums up, in a fixed order, while they go on.
+#include <atomic>
+
 #include "../../include/qlinear_b200.h"
-#include "common.cuh"
-#include "internal.h"
+#include "bounded.cuh"
 
 namespace qlin {
 namespace {
+
+#ifndef MVCB2
+#define MVCB2 4
+#endif
+constexpr int KB = 128;                // k of a block: one weight scale, one exponent
+constexpr int WARPS = 8;               // that multiply
+constexpr int THREADS = 32 * (WARPS + 3);
+// Bytes of weights a stage, 2 or 1 blocks of 128 k a warp: with few columns
+// the larger, whose fixed costs are half (the digits of eight rows leave no
+// room for it).
+template <int CB> constexpr int kStage = CB <= 2 ? 32768 : 16384;
+// Buffers of partial sums between the multiplying warps and the one that adds them up.
+template <int CB> constexpr int kParts = CB <= 2 ? 3 : 2;
+constexpr int MAX_STAGES = 12;
+constexpr int AHEAD = 8;               // stages a multiplying warp's weight scales are read ahead, less one
+constexpr int MAX_EXPERTS = QLIN_MAX_EXPERTS;
+constexpr int SMEM = 227 * 1024;
 
 struct MatvecParams {
   const void* x;
   int64_t Rx, ldx;
   const uint8_t* w;       // [E, N, K / 2]
   const void* scale;      // [E, N, groups]
-  int scale_dt;
+  int scale_bf16;
   int groups;             // scales a row: K / 128, or 1
   const int32_t* offsets; // [E + 1] or null (one expert, all rows)
-  int64_t E;
+  int E;
   const int32_t* x_rows;  // [R] or null
   const void* bias;       // [E, N] or null
   void* out;              // [R, N]
-  int64_t R, N, K;
+  int R, N, K;
+  int blocks;             // of 128 k
+  int early;              // the kernel before this one is split_kernel
+  int tile;               // weight rows a stage: 32 to 256
+  int whole;              // a stage is one three-dimensional TMA box (rows are whole slabs of 128 bytes)
+  int stages;
+  int pass;               // rows of an expert whose digits fit, at most 2 * CB
+  // of split_kernel, in the caller's workspace
+  int8_t* digits;         // [Rx, blocks, half, digit, lane t, 16]
+  float* exps;            // [Rx, epitch] 2^e, negative where the row has infinities or NaN
+  int epitch;             // blocks rounded up to 4
 };
 
-// The simplest right form: one warp per output.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+__device__ __forceinline__ float scale_at(const MatvecParams& p, int64_t i) {
+  return p.scale_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.scale)[i])
+                      : __ldg(reinterpret_cast<const float*>(p.scale) + i);
+}
+// source row of result row r, or -1: a row of zeros
+__device__ __forceinline__ int64_t source_row(const MatvecParams& p, int r) {
+  const int64_t src = p.x_rows != nullptr ? (int64_t)p.x_rows[r] : r;
+  return src >= 0 && src < p.Rx ? src : -1;
+}
+
+// ---------------------------------------------------------------------------
+// activations -> digits
+// ---------------------------------------------------------------------------
+
+// One block a row, a warp 128 k at a time; lane l has k 4l .. 4l + 3 of them.
+// The matrix instruction meets a word of eight nibbles as its even and its
+// odd ones, so the digits of k 0 2 4 6 and of 1 3 5 7 of each eight lie
+// together; lane t of the product reads words 4t .. 4t + 3 of a block, two at
+// a time.
 template <int DT>
-__global__ void __launch_bounds__(256) matvec_simple_kernel(MatvecParams p) {
+__global__ void __launch_bounds__(1024) split_kernel(MatvecParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t o = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (o >= p.R * p.N) return;
-  const int64_t r = o / p.N, n = o % p.N;
-  int64_t e = 0;
-  if (p.offsets != nullptr) {
-    int64_t begin = max(0, p.offsets[0]);
-    e = -1;
-    if (r >= begin) {
-      for (int64_t i = 0; i < p.E; ++i) {
-        const int64_t end = max(begin, (int64_t)p.offsets[i + 1]);
-        if (r < end) { e = i; break; }
-        begin = end;
-      }
-    }
-  }
-  typename Elem<DT>::T* out = reinterpret_cast<typename Elem<DT>::T*>(p.out) + o;
-  if (e < 0) {
-    if (lane == 0) *out = Elem<DT>::from_f(0.0f);
-    return;
-  }
-  const int64_t src = p.x_rows != nullptr ? (int64_t)p.x_rows[r] : r;
-  const int64_t row = e * p.N + n;
-  float acc = 0.0f;
-  if (src >= 0 && src < p.Rx) {
-    const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + src * p.ldx;
-    const int64_t glen = p.K / p.groups;
-    for (int g = 0; g < p.groups; ++g) {
-      float part = 0.0f;
-      for (int64_t b = g * glen / 2 + lane; b < (g + 1) * glen / 2; b += 32) {
-        const int c = (int)p.w[row * (p.K / 2) + b];
-        part = __fmaf_rn(Elem<DT>::to_f(x[2 * b]), (float)(((c & 15) ^ 8) - 8), part);
-        part = __fmaf_rn(Elem<DT>::to_f(x[2 * b + 1]), (float)((c >> 4 ^ 8) - 8), part);
-      }
-      const int64_t si = row * p.groups + g;
-      const float s = p.scale_dt == DT_F32 ? reinterpret_cast<const float*>(p.scale)[si]
-                                           : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.scale)[si]);
-      acc = __fmaf_rn(part, s, acc);
-    }
-  }
+  const int64_t r = blockIdx.x;
+  const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + r * p.ldx;
+  bool odd = false;
+  for (int b = warp; b < p.blocks; b += blockDim.x >> 5) {
+    const int k = b * KB + 4 * lane;
+    float v[4];
+    uint32_t big = 0;
 #pragma unroll
-  for (int o2 = 16; o2 > 0; o2 >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o2);
-  if (lane == 0) {
-    if (p.bias != nullptr) acc += Elem<DT>::to_f(reinterpret_cast<const typename Elem<DT>::T*>(p.bias)[row]);
-    *out = Elem<DT>::from_f(acc);
+    for (int i = 0; i < 4; ++i) {
+      v[i] = k + i < p.K ? Elem<DT>::to_f(x[k + i]) : 0.0f;
+      if (!(fabsf(v[i]) <= 3.402823466e38f)) {  // added separately, see odd_terms
+        odd = true;
+        v[i] = 0.0f;
+      }
+      big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    }
+    big = __reduce_max_sync(0xffffffffu, big);
+    const int e = max((int)(big >> 23), 1) - 127;  // |x| < 2^(e + 1)
+    // 2^(29 - e) in two factors, each a float
+    const float f1 = pow2((29 - e) >> 1), f2 = pow2(29 - e - ((29 - e) >> 1));
+    uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit q of the four k
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int X = __float2int_rn(__fmul_rn(__fmul_rn(v[i], f1), f2));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int digit = (int)(int8_t)(X & 0xFF);
+        d[q] |= ((uint32_t)digit & 0xFFu) << (8 * i);
+        X = (X - digit) >> 8;
+      }
+    }
+    const int word = lane >> 1;  // of eight k
+    uint8_t* out = reinterpret_cast<uint8_t*>(p.digits) + (r * p.blocks + b) * (4 * KB) + (word >> 1 & 1) * 256 +
+                   (word >> 2) * 16 + (word & 1) * 8 + 2 * (lane & 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      *reinterpret_cast<uint16_t*>(out + q * 64) = (uint16_t)__byte_perm(d[q], 0u, 0x4420);      // k 0, 2
+      *reinterpret_cast<uint16_t*>(out + q * 64 + 4) = (uint16_t)__byte_perm(d[q], 0u, 0x4431);  // k 1, 3
+    }
+    if (lane == 0) p.exps[r * p.epitch + b] = pow2(e);
   }
+  if (__syncthreads_or(odd))
+    for (int b = threadIdx.x; b < p.blocks; b += blockDim.x) p.exps[r * p.epitch + b] *= -1.0f;
+}
+
+// What the infinities and NaN of a row add to one output.
+template <int DT>
+__device__ float odd_terms(const MatvecParams& p, int64_t src, int64_t row) {
+  const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + src * p.ldx;
+  float v = 0.0f;
+  for (int k = 0; k < p.K; ++k) {
+    const float f = Elem<DT>::to_f(x[k]);
+    if (fabsf(f) <= 3.402823466e38f) continue;
+    const int c = p.w[row * (p.K >> 1) + (k >> 1)] >> (4 * (k & 1)) & 15;
+    v += __fmul_rn(f, __fmul_rn((float)((c ^ 8) - 8), p.groups > 1 ? scale_at(p, row * p.groups + k / KB) : 1.0f));
+  }
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// digits x weights
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct Smem {  // behind the ring, the digits, the partial sums and the scales
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], pfull[3], pempty[3], xfull, xempty;
+  int abort_flag;
+  int begin[MAX_EXPERTS + 1];  // first row of each expert, ascending within [0, R]
+  int cum[MAX_EXPERTS + 1];    // passes before each expert's
+};
+
+// An item of work: one row tile of one pass (up to p.pass rows of an expert).
+// Items are numbered pass by pass, and a block of threads has consecutive
+// ones, so that it changes its digits seldom.
+struct Item {
+  int left;                // items of this block from here on
+  int pass, e, r0, rows, n0;
+  __device__ __forceinline__ void find(const MatvecParams& p, const Smem* s) {
+    while (s->cum[e + 1] <= pass) ++e;  // passes ascend
+    const int r = (pass - s->cum[e]) * p.pass;
+    r0 = s->begin[e] + r;
+    rows = min(p.pass, s->begin[e + 1] - r0);
+  }
+  __device__ __forceinline__ void start(const MatvecParams& p, const Smem* s) {
+    const int tiles = (p.N + p.tile - 1) / p.tile;
+    const int64_t items = (int64_t)s->cum[p.E] * tiles;
+    const int first = (int)(items * blockIdx.x / gridDim.x);
+    left = (int)(items * (blockIdx.x + 1) / gridDim.x) - first;
+    pass = first / tiles;
+    n0 = (first - pass * tiles) * p.tile;
+    e = 0;
+    if (left > 0) find(p, s);
+  }
+  __device__ __forceinline__ void next(const MatvecParams& p, const Smem* s) {
+    --left;
+    n0 += p.tile;
+    if (n0 >= p.N) {
+      n0 = 0;
+      ++pass;
+      if (left > 0) find(p, s);
+    }
+  }
+};
+
+__device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Everything read before pdl_wait was complete before split_kernel let this
+// kernel start (it waits for the kernels before it first).
+// CB: blocks of 8 columns, two rows each.
+template <int DT, int CB, bool GROUPS>
+__global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constant__ CUtensorMap tmW, MatvecParams p) {
+  using T = typename Elem<DT>::T;
+  constexpr int STAGE = kStage<CB>, BLK = STAGE / 16384;  // blocks of 128 k a warp and stage
+  constexpr int PARTS = kParts<CB>;
+  constexpr int PITCH = 2 * CB + 1;                       // of a warp's partial sums [32 rows][PITCH]
+  constexpr int PART = 32 * PITCH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xdig = ring + p.stages * STAGE;                            // [pass][blocks][512]
+  float* xexp = reinterpret_cast<float*>(xdig + (int64_t)p.pass * p.blocks * (4 * KB));  // [pass][epitch]
+  float* part = xexp + p.pass * p.epitch;                             // [PARTS][WARPS][PART]
+  // words that hold the scales of a stage: [AHEAD][warp][block][lane g][row of four]
+  uint32_t(*scales)[WARPS][BLK][32] = reinterpret_cast<uint32_t(*)[WARPS][BLK][32]>(part + PARTS * WARPS * PART);
+  Smem* s = reinterpret_cast<Smem*>(scales + AHEAD);
+  volatile int* abort_flag = &s->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&s->full[i], 1);
+      mbar_init(&s->empty[i], WARPS);
+    }
+    for (int i = 0; i < PARTS; ++i) {
+      mbar_init(&s->pfull[i], WARPS);
+      mbar_init(&s->pempty[i], 1);
+    }
+    mbar_init(&s->xfull, 1);
+    mbar_init(&s->xempty, WARPS + 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  if (!p.early) pdl_wait();
+  if (p.offsets != nullptr) {
+    for (int e = threadIdx.x; e <= p.E; e += THREADS) s->begin[e] = min(max(p.offsets[e], 0), p.R);
+  } else if (threadIdx.x < 2) {
+    s->begin[threadIdx.x] = threadIdx.x ? p.R : 0;
+  }
+  __syncthreads();
+  if (warp == 0) expert_bounds(s->begin, s->cum, p.E, lane, [&](int rows) { return (rows + p.pass - 1) / p.pass; });
+  __syncthreads();
+  const int slabs = STAGE / (128 * p.tile);                    // of 128 bytes a row and stage
+  const int steps = (p.blocks + 2 * slabs - 1) / (2 * slabs);  // stages of a tile
+  const int row_groups = p.tile >> 5;                          // of 32 rows
+  const int share = WARPS / row_groups;                        // warps of a row group
+
+  if (warp == WARPS) {
+    // ---------------- weights ----------------
+    if (lane == 0) {
+      tma_prefetch_desc(&tmW);
+      int stage = 0;
+      uint32_t phase = 0;
+      Armed armed;
+      bool ok = true;
+      Item it;
+      for (it.start(p, s); it.left > 0 && ok; it.next(p, s)) {
+        const int row = it.e * p.N + it.n0;
+        for (int st = 0; st < steps; ++st) {
+          if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          mbar_arrive_expect_tx(&s->full[stage], STAGE);
+          uint8_t* d = ring + stage * STAGE;
+          if (p.whole) {
+            tma_load_3d(d, &tmW, &s->full[stage], 0, row, st * slabs);
+          } else {
+            for (int i = 0; i < slabs; ++i)  // (behind K: zeros)
+              tma_load_2d(d + i * 128 * p.tile, &tmW, &s->full[stage], (st * slabs + i) * 128, row);
+          }
+          armed.note(stage, phase);
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      armed.drain(s->full);  // no load still writing shared memory at exit
+    }
+  } else if (warp == WARPS + 1) {
+    // ---------------- digits and exponents of a pass's rows ----------------
+    if (p.early) pdl_wait();
+    int now = -1;
+    uint32_t loads = 0;
+    Item it;
+    for (it.start(p, s); it.left > 0; it.next(p, s)) {
+      if (it.pass == now) continue;
+      now = it.pass;
+      bool ok = true;
+      if (lane == 0 && loads > 0) ok = wait_bounded(&s->xempty, (loads - 1) & 1, abort_flag);
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+      const int64_t src = lane < it.rows ? source_row(p, it.r0 + lane) : -1;
+      const uint32_t live = __ballot_sync(0xffffffffu, src >= 0);
+      if (lane < it.rows && src < 0)  // a row of zeros: whatever its digits are
+        for (int i = 0; i < p.epitch; ++i) xexp[lane * p.epitch + i] = 0.0f;
+      __syncwarp();
+      const uint32_t dbytes = (uint32_t)p.blocks * (4 * KB), ebytes = (uint32_t)p.epitch * 4;
+      if (lane == 0) mbar_arrive_expect_tx(&s->xfull, (uint32_t)__popc(live) * (dbytes + ebytes));
+      __syncwarp();
+      if (src >= 0) {
+        bulk_load(xdig + (int64_t)lane * dbytes, p.digits + src * dbytes, dbytes, &s->xfull);
+        bulk_load(xexp + lane * p.epitch, p.exps + src * p.epitch, ebytes, &s->xfull);
+      }
+      ++loads;
+    }
+    if (lane == 0 && loads > 0) wait_drain(&s->xfull, (loads - 1) & 1);
+  } else if (warp == WARPS + 2) {
+    // ---------------- outputs ----------------
+    if (p.early) pdl_wait();  // before anything is written
+    {  // rows of no expert
+      const int64_t line = (int64_t)p.N * sizeof(T);
+      const int64_t thread = (int64_t)blockIdx.x * 32 + lane, count = (int64_t)gridDim.x * 32;
+      if (s->begin[0] > 0) zero_bytes(p.out, 0, s->begin[0] * line, thread, count);
+      if (s->begin[p.E] < p.R) zero_bytes(p.out, s->begin[p.E] * line, p.R * line, thread, count);
+    }
+    int buf = 0, now = -1;
+    uint32_t phase = 0;
+    Item it;
+    for (it.start(p, s); it.left > 0; it.next(p, s)) {
+      if (it.pass != now) {
+        if (now >= 0) {  // done with the exponents of the pass before
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s->xempty);
+        }
+        now = it.pass;
+      }
+      // bias and scale of this lane's column of each 32, read before the sums are waited for
+      constexpr int MAXG = 8;
+      float bias[MAXG], row_scale[MAXG];
+#pragma unroll
+      for (int j = 0; j < MAXG; ++j) {
+        bias[j] = 0.0f;
+        row_scale[j] = 1.0f;
+        if (j < row_groups) {
+          const int64_t at = (int64_t)it.e * p.N + min(it.n0 + 32 * j + lane, p.N - 1);
+          if (p.bias != nullptr) bias[j] = Elem<DT>::to_f(reinterpret_cast<const T*>(p.bias)[at]);
+          if constexpr (!GROUPS) row_scale[j] = scale_at(p, at);
+        }
+      }
+      if (!wait_bounded(&s->pfull[buf], phase, abort_flag)) break;
+      for (int j = 0; j < row_groups; ++j) {
+        const int n = it.n0 + 32 * j + lane;
+        if (n < p.N) {
+          float b = bias[0], rs = row_scale[0];
+#pragma unroll
+          for (int i = 1; i < MAXG; ++i)
+            if (i == j) { b = bias[i]; rs = row_scale[i]; }
+          const int64_t at = (int64_t)it.e * p.N + n;
+          for (int r = 0; r < it.rows; ++r) {
+            const float* q = part + (buf * WARPS + j) * PART + lane * PITCH + r;
+            float v = 0.0f;
+            for (int k = 0; k < share; ++k) v += q[k * row_groups * PART];
+            if (xexp[r * p.epitch] < 0.0f) v += odd_terms<DT>(p, source_row(p, it.r0 + r), at);
+            if constexpr (!GROUPS) v *= rs;
+            if (p.bias != nullptr) v += b;
+            reinterpret_cast<T*>(p.out)[(int64_t)(it.r0 + r) * p.N + n] = Elem<DT>::from_f(v);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->pempty[buf]);
+      if (++buf == PARTS) { buf = 0; phase ^= 1; }
+    }
+  } else {
+    // ---------------- products ----------------
+    const int g = lane >> 2, t = lane & 3;
+    const int rg = warp & (row_groups - 1);           // this warp's row group,
+    const int bi = warp / row_groups * BLK;           // and its first block of a stage
+    // lane group g has rows r = g/2 + 4 (g%2) and r + 8 of each 16: rows 4
+    // apart lie in different halves of the 128-byte swizzle's banks
+    const int row = (g >> 1) + 4 * (g & 1);
+    uint32_t woff[BLK];
+#pragma unroll
+    for (int k = 0; k < BLK; ++k)
+      woff[k] = (uint32_t)(((bi + k) >> 1) * 128 * p.tile + (rg * 32 + row) * 128 + (((((bi + k) & 1) * 4 + t) ^ row) * 16));
+    // 16 q times digit d of X = x 2^(29 - e): lanes of odd t have the upper two digits
+    const float unit = (t & 1) ? pow2(16 - 33) : pow2(-33);
+    // rows behind the last of a pass repeat it (their sums are not stored)
+    auto xrow = [&](int c, int odd_half, int rows) { return min(2 * c + odd_half, rows - 1); };
+
+    // Weight scales are copied (cp.async) AHEAD - 1 stages before their use: of
+    // the four rows of lane group g lane t copies row 8 t, and all four lanes
+    // read them back.  A scale read into a register an iteration ahead
+    // stalled each stage for the memory's latency.
+    Item pf;
+    int pf_step = 0, pf_slot = 0;
+    int64_t pf_row = 0;
+    pf.start(p, s);
+    auto fetch = [&]() {
+      if constexpr (GROUPS) {
+        if (pf.left > 0) {
+          if (pf_step == 0) pf_row = ((int64_t)pf.e * p.N + min(pf.n0 + rg * 32 + 8 * t + row, p.N - 1)) * p.groups;
+          const int b = pf_step * 2 * slabs + bi;
+          const uint8_t* from = static_cast<const uint8_t*>(p.scale) + (pf_row + b) * (p.scale_bf16 ? 2 : 4);
+#pragma unroll
+          for (int k = 0; k < BLK; ++k)
+            if (b + k < p.blocks)
+              cp_async_4(&scales[pf_slot][warp][k][lane],
+                         reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(from + k * (p.scale_bf16 ? 2 : 4)) & ~uintptr_t(3)));
+          if (++pf_step == steps) {
+            pf_step = 0;
+            pf.next(p, s);
+          }
+        }
+        cp_async_commit();
+        pf_slot = (pf_slot + 1) & (AHEAD - 1);
+      }
+    };
+    for (int i = 0; i < AHEAD - 1; ++i) fetch();
+    int stage = 0, now = -1, buf = 0, slot = 0;
+    uint32_t phase = 0, loads = 0, pphase = 0;
+    bool ok = true;
+    Item it;
+    for (it.start(p, s); it.left > 0 && ok; it.next(p, s)) {
+      if (it.pass != now) {
+        if (now >= 0) {  // this warp is done with the digits of the pass before
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s->xempty);
+        }
+        now = it.pass;
+        ok = wait_bounded(&s->xfull, loads & 1, abort_flag);
+        ++loads;
+      }
+      const uint8_t* xd[CB];
+      const float* xe[CB];
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        xd[c] = xdig + (int64_t)xrow(c, g >> 2, it.rows) * p.blocks * (4 * KB) + (g & 3) * 64 + t * 16;
+        xe[c] = xexp + xrow(c, t >> 1, it.rows) * p.epitch;
+      }
+      uint32_t upper = 0;  // bit j: the bfloat16 scale of row j and block 0 is a word's upper half
+      if (GROUPS && p.scale_bf16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t first = ((int64_t)it.e * p.N + min(it.n0 + rg * 32 + 8 * j + row, p.N - 1)) * p.groups;
+          upper |= ((uint32_t)(reinterpret_cast<uintptr_t>(p.scale) >> 1) + (uint32_t)first & 1u) << j;
+        }
+      }
+      float sum[2][CB][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) sum[i][c][0] = sum[i][c][1] = 0.0f;
+#pragma unroll 1
+      for (int st = 0; st < steps && ok; ++st) {
+        const int b0 = st * 2 * slabs + bi;
+        if constexpr (GROUPS) {
+          fetch();
+          cp_async_wait<AHEAD - 1>();
+          __syncwarp();
+        }
+        if (!wait_bounded(&s->full[stage], phase, abort_flag)) { ok = false; break; }
+#pragma unroll
+        for (int k = 0; k < BLK; ++k) {
+          const int b = b0 + k;
+          if (b >= p.blocks) break;
+          float ws[2][2] = {{unit, unit}, {unit, unit}};
+          if constexpr (GROUPS) {
+            const uint4 u = *reinterpret_cast<const uint4*>(&scales[slot][warp][k][lane & ~3]);
+            const uint32_t word[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float f = __uint_as_float(word[j]);
+              if (p.scale_bf16) f = __uint_as_float((upper >> j ^ b) & 1u ? word[j] & 0xFFFF0000u : word[j] << 16);
+              ws[j >> 1][j & 1] = __fmul_rn(f, unit);
+            }
+          }
+          const uint8_t* d = ring + stage * STAGE + woff[k];
+          uint4 w[2][2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[i][h] = *reinterpret_cast<const uint4*>(d + (16 * i + 8 * h) * 128);
+          int acc[2][CB][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[i][c][j] = 0;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint4 xv[CB];
+#pragma unroll
+            for (int c = 0; c < CB; ++c) xv[c] = *reinterpret_cast<const uint4*>(xd[c] + b * (4 * KB) + half * 256);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {  // a word of eight k a lane
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint32_t a[2][2];  // [row half][even, odd k]: 16 times the nibble
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t u = half == 0 ? (q == 0 ? w[i][h].x : w[i][h].y) : (q == 0 ? w[i][h].z : w[i][h].w);
+                  a[h][0] = (u << 4) & 0xF0F0F0F0u;
+                  a[h][1] = u & 0xF0F0F0F0u;
+                }
+#pragma unroll
+                for (int c = 0; c < CB; ++c)
+                  mma16832(acc[i][c], a[0][0], a[1][0], a[0][1], a[1][1], q ? xv[c].z : xv[c].x, q ? xv[c].w : xv[c].y);
+              }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < CB; ++c) {
+            const float xs = fabsf(xe[c][b]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                // |digit sums| <= 128 * 128 * 128: both digits fit an int
+                const float v = __int2float_rn(acc[i][c][2 * h] + 256 * acc[i][c][2 * h + 1]);
+                sum[i][c][h] = __fmaf_rn(__fmul_rn(v, ws[i][h]), xs, sum[i][c][h]);
+              }
+          }
+        }
+        slot = (slot + 1) & (AHEAD - 1);
+        __syncwarp();  // (also: the slot read above may be copied to again)
+        if (lane == 0) mbar_arrive(&s->empty[stage]);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok || !wait_bounded(&s->pempty[buf], pphase ^ 1, abort_flag)) break;
+      float* to = part + (buf * WARPS + warp) * PART;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float v = sum[i][c][h] + __shfl_xor_sync(0xffffffffu, sum[i][c][h], 1);
+            if (!(t & 1)) to[(16 * i + 8 * h + row) * PITCH + 2 * c + (t >> 1)] = v;
+          }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->pfull[buf]);
+      if (++buf == PARTS) { buf = 0; pphase ^= 1; }
+    }
+    if constexpr (GROUPS) cp_async_wait<0>();
+  }
+}
+
+// The same for any K and alignment, digits and weights straight from memory:
+// one warp 16 weight rows and 2 rows of one expert (grid.y: the experts that
+// have rows, one after another).
+template <int DT, bool GROUPS>
+__global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) {
+  using T = typename Elem<DT>::T;
+  __shared__ int s_begin[MAX_EXPERTS + 1], s_cum[MAX_EXPERTS + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (p.offsets != nullptr) {
+    for (int e = threadIdx.x; e <= p.E; e += 32 * WARPS) s_begin[e] = min(max(p.offsets[e], 0), p.R);
+  } else if (threadIdx.x < 2) {
+    s_begin[threadIdx.x] = threadIdx.x ? p.R : 0;
+  }
+  __syncthreads();
+  if (warp == 0) expert_bounds(s_begin, s_cum, p.E, lane, [](int rows) { return rows > 0; });
+  __syncthreads();
+  {
+    const int64_t line = (int64_t)p.N * sizeof(T), block = blockIdx.y * (int64_t)gridDim.x + blockIdx.x;
+    const int64_t thread = block * 32 * WARPS + threadIdx.x, count = (int64_t)gridDim.x * gridDim.y * 32 * WARPS;
+    if (s_begin[0] > 0) zero_bytes(p.out, 0, s_begin[0] * line, thread, count);
+    if (s_begin[p.E] < p.R) zero_bytes(p.out, s_begin[p.E] * line, p.R * line, thread, count);
+  }
+  if ((int)blockIdx.y >= s_cum[p.E]) return;
+  int e = 0;
+  while (s_cum[e + 1] <= (int)blockIdx.y) ++e;
+  const int n0 = (blockIdx.x * WARPS + warp) * 16, bytes = p.K >> 1;
+  if (n0 >= p.N) return;
+  const float unit = (t & 1) ? pow2(16 - 33) : pow2(-33);
+  const int64_t wrow[2] = {(int64_t)e * p.N + min(n0 + g, p.N - 1), (int64_t)e * p.N + min(n0 + 8 + g, p.N - 1)};
+  for (int r0 = s_begin[e]; r0 < s_begin[e + 1]; r0 += 2) {
+    const int rows = min(2, s_begin[e + 1] - r0);
+    const int64_t src = source_row(p, min(r0 + (g >> 2), r0 + rows - 1));  // whose digits this lane reads
+    const int64_t sum_src = source_row(p, min(r0 + (t >> 1), r0 + rows - 1));  // whose sums it gets
+    float sum[2] = {0.0f, 0.0f};
+    for (int b = 0; b < p.blocks; ++b) {
+      int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t a[2][2];
+        const int at = b * (KB / 2) + 16 * t + 4 * q;  // byte of the row
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t u = 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at + i < bytes) u |= (uint32_t)p.w[wrow[h] * bytes + at + i] << (8 * i);
+          a[h][0] = (u << 4) & 0xF0F0F0F0u;
+          a[h][1] = u & 0xF0F0F0F0u;
+        }
+        uint2 v = make_uint2(0u, 0u);
+        if (src >= 0)
+          v = *reinterpret_cast<const uint2*>(p.digits + (src * p.blocks + b) * (4 * KB) + (q >> 1) * 256 + (g & 3) * 64 +
+                                              t * 16 + (q & 1) * 8);
+        mma16832(acc, a[0][0], a[1][0], a[0][1], a[1][1], v.x, v.y);
+      }
+      const float xs = sum_src >= 0 ? fabsf(p.exps[sum_src * p.epitch + b]) : 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float v = __int2float_rn(acc[2 * h] + 256 * acc[2 * h + 1]);
+        const float ws = GROUPS ? __fmul_rn(scale_at(p, wrow[h] * p.groups + b), unit) : unit;
+        sum[h] = __fmaf_rn(__fmul_rn(v, ws), xs, sum[h]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v = sum[h] + __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      const int n = n0 + 8 * h + g, r = t >> 1;
+      if ((t & 1) || r >= rows || n >= p.N) continue;
+      const int64_t at = (int64_t)e * p.N + n;
+      if (sum_src >= 0 && p.exps[sum_src * p.epitch] < 0.0f) v += odd_terms<DT>(p, sum_src, at);
+      if constexpr (!GROUPS) v *= scale_at(p, at);
+      if (p.bias != nullptr) v += Elem<DT>::to_f(reinterpret_cast<const T*>(p.bias)[at]);
+      reinterpret_cast<T*>(p.out)[(int64_t)(r0 + r) * p.N + n] = Elem<DT>::from_f(v);
+    }
+  }
+}
+
+template <int CB>
+constexpr int fixed_bytes() {
+  return 1024 + kParts<CB> * WARPS * 32 * (2 * CB + 1) * 4 + AHEAD * WARPS * (kStage<CB> / 16384) * 128 + (int)sizeof(Smem);
+}
+
+template <int DT, int CB, bool GROUPS>
+int launch_cfg(MatvecParams p, cudaStream_t stream) {
+  const int sms = device_sm_count();
+  // rows a pass: what fits beside 64 KB of weights; then as many stages as fit
+  constexpr int STAGE = kStage<CB>;
+  const int slabs = (p.K / 2 + 127) / 128;  // of 128 bytes a row; as few rows a tile as fill whole stages: the most tiles to share out
+  p.tile = 32;
+  while (p.tile < 8 * 32 && STAGE / (128 * p.tile) > slabs) p.tile *= 2;
+  p.whole = p.K % 256 == 0 && STAGE > 128 * p.tile;  // one slab a stage: the map stays two-dimensional
+  const int64_t room = SMEM - fixed_bytes<CB>(), per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
+  const int64_t fit = (room - 65536) / per_row;
+  p.pass = (int)(fit < 2 * CB ? fit : 2 * CB);
+  if (p.pass > p.R) p.pass = p.R;
+  const int64_t stages = (room - p.pass * per_row) / STAGE;
+  p.stages = (int)(stages < MAX_STAGES ? stages : MAX_STAGES);
+  const int64_t passes = p.R / p.pass + (p.offsets == nullptr ? 1 : (p.R < p.E ? p.R : p.E));  // at most
+  const int64_t items = passes * ((p.N + p.tile - 1) / p.tile);
+  if (items > INT32_MAX) return fail(QLIN_ERR_UNSUPPORTED, "matvec_w4: too many outputs");
+  CUtensorMap tw;
+  const int rc = encode_slab_tmap(&tw, p.w, (uint64_t)p.K / 2, (uint64_t)p.E * p.N, 128, p.tile,
+                                  p.whole ? STAGE / (128 * p.tile) : 1);
+  if (rc) return rc;
+  auto kern = matvec_kernel<DT, CB, GROUPS>;
+  static std::atomic<uint64_t> attr_devices{0};  // shared-memory limit raised once per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  cudaError_t e;
+  if (!(attr_devices.load() & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(matvec_w4)");
+    attr_devices.fetch_or(bit);
+  }
+  e = launch_pdl(kern, dim3((unsigned)(items < sms ? items : sms)), dim3(THREADS),
+                 (size_t)(fixed_bytes<CB>() + p.pass * per_row + p.stages * STAGE), stream, tw, p);
+  return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
+}
+
+template <int DT, int CB>
+int launch_cb(const MatvecParams& p, cudaStream_t stream) {
+  return p.groups > 1 ? launch_cfg<DT, CB, true>(p, stream) : launch_cfg<DT, CB, false>(p, stream);
+}
+
+template <int DT>
+int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
+  cudaError_t e;
+  if (p.early) {
+    const int threads = 32 * (p.blocks < 32 ? p.blocks : 32);
+    e = launch_pdl(split_kernel<DT>, dim3((unsigned)p.Rx), dim3(threads), 0, stream, p);
+    if (e != cudaSuccess) return cuda_fail(e, "matvec_w4 split launch");
+  }
+  const int64_t per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
+  if (!aligned || per_row > SMEM - fixed_bytes<4>() - 65536) {  // (the latter: K above 34,000)
+    const int64_t slots = p.offsets == nullptr ? 1 : (p.R < p.E ? p.R : p.E);
+    const dim3 grid((unsigned)((p.N + 16 * WARPS - 1) / (16 * WARPS)), (unsigned)slots), block(32 * WARPS);
+    e = p.groups > 1 ? launch_pdl(matvec_any_kernel<DT, true>, grid, block, 0, stream, p)
+                     : launch_pdl(matvec_any_kernel<DT, false>, grid, block, 0, stream, p);
+    return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
+  }
+  // rows an expert, on average: how they spread is known on the device only
+  const int64_t rows = p.offsets == nullptr ? p.R : (p.R < p.E ? 1 : p.R / p.E);
+  if (rows <= 2) return launch_cb<DT, 1>(p, stream);
+  if (rows <= MVCB2) return launch_cb<DT, 2>(p, stream);
+  return launch_cb<DT, 4>(p, stream);
+}
+
+struct Workspace {
+  int64_t blocks, epitch;
+  size_t exps, bytes;
+};
+Workspace workspace_layout(int64_t Rx, int64_t K) {
+  Workspace w;
+  w.blocks = (K + KB - 1) / KB;
+  w.epitch = (w.blocks + 3) & ~int64_t(3);
+  w.exps = (size_t)(Rx * w.blocks * (4 * KB));
+  w.bytes = w.exps + (size_t)(Rx * w.epitch) * sizeof(float);
+  return w;
 }
 
 }  // namespace
 
+size_t matvec_workspace_bytes(int64_t Rx, int64_t K) { return workspace_layout(Rx, K).bytes; }
+
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
-                     int64_t R, int64_t N, int64_t K, cudaStream_t stream) {
-  const MatvecParams p{x, Rx, ldx, w, scale, scale_dt, groups, offsets, E, x_rows, bias, out, R, N, K};
-  const int64_t blocks = (R * N + 7) / 8;
-  if (blocks > INT32_MAX) return fail(QLIN_ERR_UNSUPPORTED, "matvec_w4: too many outputs");
-  const dim3 grid((unsigned)blocks), block(256);
-  cudaError_t e;
-  if (dt == DT_BF16) e = launch_pdl(matvec_simple_kernel<DT_BF16>, grid, block, 0, stream, p);
-  else if (dt == DT_F16) e = launch_pdl(matvec_simple_kernel<DT_F16>, grid, block, 0, stream, p);
-  else e = launch_pdl(matvec_simple_kernel<DT_F32>, grid, block, 0, stream, p);
-  return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
+                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream) {
+  if (device_sm_count() < 1) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
+  const Workspace l = workspace_layout(Rx, K);
+  MatvecParams p{};
+  p.x = x;
+  p.Rx = Rx;
+  p.ldx = ldx;
+  p.w = w;
+  p.scale = scale;
+  p.scale_bf16 = scale_dt == DT_BF16;
+  p.groups = groups;
+  p.offsets = offsets;
+  p.E = (int)E;
+  p.x_rows = x_rows;
+  p.bias = bias;
+  p.out = out;
+  p.R = (int)R;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.blocks = (int)l.blocks;
+  p.early = Rx > 0;
+  p.digits = static_cast<int8_t*>(workspace);
+  p.exps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + l.exps);
+  p.epitch = (int)l.epitch;
+  const bool aligned = K % 32 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  if (dt == DT_BF16) return launch_dt<DT_BF16>(p, aligned, stream);
+  if (dt == DT_F16) return launch_dt<DT_F16>(p, aligned, stream);
+  return launch_dt<DT_F32>(p, aligned, stream);
 }
+
+int set_matvec_wait_limit(uint64_t ns) { return set_tu_wait_limit(ns); }
+int read_matvec_error(cudaStream_t stream, uint32_t* bits) { return read_tu_error(stream, bits); }
 
 }  // namespace qlin

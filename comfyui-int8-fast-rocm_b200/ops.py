@@ -823,9 +823,9 @@ def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=Non
 
 
 def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
-    """Linear of few rows with packed 4-bit weights, the activations kept in
-    their dtype: ``y = dt(x @ (q * scale).T + bias)`` with float32 sums and
-    one rounding.  ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in
+    """Linear of few rows with packed 4-bit weights, the activations not
+    quantised: ``y = dt(x @ (q * scale).T + bias)`` with exact sums of each
+    128 k, float32 sums of those, and one rounding (see qlin_matvec_w4).  ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in
     place), ``w_packed`` [N, K/2] and ``w_scale`` [N] (or [N, 1]) or
     [N, K/128], float32 or bfloat16, as :func:`quant_weight_int4` returns
     them; ``bias`` [N]; the result is in x.dtype.
@@ -836,7 +836,7 @@ def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     :func:`gemm_w8a8_grouped`).  ``x_rows`` [R] gathers: result row r takes
     row ``x_rows[r]`` of ``x`` (an index outside [0, Rx) is a row of zeros).
 
-    The weights are read once for each 32 rows of an expert; many rows are
+    The weights are read once for each 2 to 8 rows of an expert; many rows are
     :func:`gemm_w4_g128`'s and :func:`gemm_w8a8_grouped`'s work."""
     if w_packed.dtype != torch.int8:
         raise TypeError("packed int4 weights are int8 tensors")
@@ -876,9 +876,12 @@ def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     st = _stream(x)
     out = torch.empty((R, Nn), dtype=x.dtype, device=dev)
     if R and Nn:
+        need = ctypes.c_uint64(0)
+        N.call("qlin_matvec_w4_workspace", Rx, K, ctypes.addressof(need))
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)  # freed (in stream order) with the call
         N.call("qlin_matvec_w4", x.data_ptr(), dt, Rx, max(ldx, K), w_packed.data_ptr(), w_scale.data_ptr(),
                dtype_code(w_scale.dtype), 128 if groups else 0, _ptr(offsets), E, _ptr(x_rows), _ptr(bias),
-               out.data_ptr(), R, Nn, K, st)
+               out.data_ptr(), R, Nn, K, ws.data_ptr(), need.value, st)
     return out
 
 

@@ -469,21 +469,27 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
                                     const void* bias, void* out, int out_dtype, int64_t R, int64_t N, int64_t K,
                                     void* workspace, uint64_t workspace_bytes, void* stream);
 
-/* Few rows times packed 4-bit weights, the activations kept in their dtype:
+/* Few rows times packed 4-bit weights, the activations not quantised:
  *   out[r, n] = dt(sum_g w_scale[n, g] * (sum_{k in g} x[src(r), k] * q[n, k]) + bias[n])
- * with float32 sums and one rounding; q signed nibbles [N, K/2] (low nibble =
- * even k), group 128 (K % 128 == 0) or 0 (one scale a row, any even K), the
- * layouts of qlin_quant_weight_int4; w_scale F32 or BF16.  x [Rx, K] (row
- * stride ldx) and bias [N] in x_dtype, out [R, N] in x_dtype.
+ * with one rounding; q signed nibbles [N, K/2] (low nibble = even k), group
+ * 128 (K % 128 == 0) or 0 (one scale a row, any even K), the layouts of
+ * qlin_quant_weight_int4; w_scale F32 or BF16.  x [Rx, K] (row stride ldx)
+ * and bias [N] in x_dtype, out [R, N] in x_dtype.  Each 128 k are summed
+ * exactly, with x as 32-bit integers in units of 2^-30 of their largest
+ * (which 16-bit values are, exactly, down to 2^-19 of it); the sums of the
+ * 128 are scaled and added in float32.
  * offsets NULL: E == 1, all rows use the one weight.  Otherwise w_packed
  * [E, N, K/2], w_scale [E, N, G] and bias [E, N], rows sorted by expert; rows
  * of no expert become 0.  src(r) = x_rows ? x_rows[r] : r; a source row
  * outside [0, Rx) counts as a row of zeros.  Any R works; the weights are read
- * once for each 32 rows of an expert, so many rows belong to the GEMMs. */
+ * once for each 2 to 8 rows of an expert, so many rows belong to the GEMMs.
+ * workspace: qlin_matvec_w4_workspace(Rx, K) bytes of device memory, 16-byte
+ * aligned, used within the call only (NULL when Rx is 0). */
+QLIN_API int qlin_matvec_w4_workspace(int64_t Rx, int64_t K, uint64_t* bytes);
 QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,
                             const void* w_scale, int scale_dtype, int group, const int32_t* offsets, int64_t E,
                             const int32_t* x_rows, const void* bias, void* out, int64_t R, int64_t N, int64_t K,
-                            void* stream);
+                            void* workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

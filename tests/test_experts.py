@@ -446,6 +446,12 @@ def test_matvec_layouts(pkg):
     assert_matvec(got, *matvec_ref(x, p, s, b, None, None), 384)
     got = pkg.ops.matvec_w4(x.cuda(), p.cuda(), s.T.contiguous().cuda().T, b.cuda())
     assert torch.equal(got, want)
+    half = s.to(torch.bfloat16)
+    for at in (0, 1, 2, 3):  # two-byte scales off a word, three a row
+        buf = torch.zeros(50 * 3 + 3, dtype=torch.bfloat16).cuda()
+        buf[at:at + 150] = half.cuda().reshape(-1)
+        got = pkg.ops.matvec_w4(x.cuda(), p.cuda(), buf[at:at + 150].view(50, 3), b.cuda())
+        assert_matvec(got, *matvec_ref(x, p, half, b, None, None), 384)
     assert pkg.ops.matvec_w4(x[:0].cuda(), p.cuda(), s.cuda(), b.cuda()).shape == (0, 50)
 
 
@@ -814,9 +820,13 @@ def test_abi_refusals(pkg):
     assert lib.qlin_gemm_w8a8_grouped_workspace(-1, 32, ctypes.addressof(n)) == bad
     assert grp(rows=16) == grp(rows=16, ws=16, nws=n.value - 16) == bad
     assert grp(rows=16, ws=8, nws=4096) == align
-    mv = lambda Rx=4, ld=256, sdt=N.F32, group=128, off=None, E=1, R=4, Nn=8, K=256, dt=N.BF16, x=16: lib.qlin_matvec_w4(
-        x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, 16, R, Nn, K, None)
+    mv = lambda Rx=4, ld=256, sdt=N.F32, group=128, off=None, E=1, R=4, Nn=8, K=256, dt=N.BF16, x=16, ws=16, nws=2 ** 20: lib.qlin_matvec_w4(
+        x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, 16, R, Nn, K, ws, nws, None)
     assert mv(E=2) == mv(E=513, off=16) == mv(R=3) == mv(K=255) == mv(ld=255) == mv(sdt=N.F16) == mv(dt=N.I8) == bad
     assert mv(K=250, ld=250) == mv(x=None) == bad
     assert mv(group=64) == unsup
     assert mv(R=0, Rx=0) == mv(Nn=0) == 0
+    assert lib.qlin_matvec_w4_workspace(4, 256, ctypes.addressof(n)) == 0 and n.value >= 4 * 256 * 4
+    assert lib.qlin_matvec_w4_workspace(-1, 256, ctypes.addressof(n)) == bad
+    assert mv(ws=None) == mv(nws=n.value - 1) == bad
+    assert mv(ws=24) == align
