@@ -5,7 +5,7 @@
 //   route    logits [T, E] -> the k best experts of every token and their
 //            weights, and the (token, slot) pairs sorted by expert;
 //   combine  out[t] = sum_j weight[t, j] * y[pos[t, j]] (+ residual[t]).
-#include <cfloat>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/qlinear_b200.h"
@@ -15,10 +15,10 @@
 namespace qlin {
 namespace {
 
-constexpr int ROUTE_THREADS = 256;
+constexpr int ROUTE_THREADS = 512;
 constexpr int ROUTE_WARPS = ROUTE_THREADS / 32;
-constexpr int ROUTE_MIN_TOKENS = 64;   // tokens of a block: 8 a warp at least
-constexpr int ROUTE_MAX_BLOCKS = 296;  // two a SM: the second kernel reads every block's counts
+constexpr int ROUTE_BLOCKS = 148;      // at most, one a SM: the second kernel's blocks read all blocks' counts
+constexpr int SORT_BATCH = 8;          // tokens whose choices a warp holds at a time
 constexpr float NEG_INF = -INFINITY;
 
 struct RouteParams {
@@ -37,21 +37,60 @@ struct RouteParams {
   int32_t* counts;    // [blocks, Ep] rows of each expert in each block
 };
 
-// Floats in the order of their values as unsigned numbers; 0 is below all.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float unordered(uint32_t u) {
-  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// A logit and its expert as one unsigned number: larger for larger logits (-0
+// as +0, NaN as -inf), for equal ones larger for lower experts; 0 is below all.
+// 16-bit logits leave room for the expert in 32 bits.
+template <int DT> struct RouteKey {
+  using T = uint64_t;
+  static __device__ __forceinline__ T make(float v, int e) {
+    const uint32_t b = __float_as_uint(v != v ? NEG_INF : v + 0.0f);
+    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFu - (uint32_t)e);
+  }
+  static __device__ __forceinline__ float value(T k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+  }
+  static __device__ __forceinline__ int expert(T k) { return (int)(0xFFFFu - ((uint32_t)k & 0xFFFFu)); }
+};
+template <int DT> struct RouteKey16 {
+  using T = uint32_t;
+  static __device__ __forceinline__ T make(float v, int e) {
+    const auto h = Elem<DT>::from_f(v != v ? NEG_INF : v + 0.0f);  // exact: v has this type
+    const uint32_t b = *reinterpret_cast<const uint16_t*>(&h);
+    return (b & 0x8000u ? ~b & 0xFFFFu : b | 0x8000u) << 16 | (0xFFFFu - (uint32_t)e);
+  }
+  static __device__ __forceinline__ float value(T k) {
+    const uint32_t u = k >> 16;
+    const uint16_t b = (uint16_t)(u & 0x8000u ? u & 0x7FFFu : ~u);
+    return Elem<DT>::to_f(*reinterpret_cast<const typename Elem<DT>::T*>(&b));
+  }
+  static __device__ __forceinline__ int expert(T k) { return (int)(0xFFFFu - (k & 0xFFFFu)); }
+};
+template <> struct RouteKey<DT_BF16> : RouteKey16<DT_BF16> {};
+template <> struct RouteKey<DT_F16> : RouteKey16<DT_F16> {};
+
 // log(1 / (1 + exp(-v))) without overflow on either side
 __device__ __forceinline__ float log_sigmoid(float v) { return fminf(v, 0.0f) - log1pf(expf(-fabsf(v))); }
+
+// The choices of SORT_BATCH tokens, slot j in lane j; -1 behind the last.
+__device__ __forceinline__ void load_choices(const RouteParams& p, int64_t t0, int64_t t1, int lane,
+                                             int (&id)[SORT_BATCH]) {
+#pragma unroll
+  for (int u = 0; u < SORT_BATCH; ++u) id[u] = lane < p.k && t0 + u < t1 ? p.ids[(t0 + u) * p.k + lane] : -1;
+}
+
+// Rows of each expert among one warp's tokens, to cnt [E] (zeros on entry).
+__device__ __forceinline__ void count_choices(const RouteParams& p, int64_t t0, int64_t t1, int lane, int32_t* cnt) {
+  for (int64_t tb = t0; tb < t1; tb += SORT_BATCH) {
+    int id[SORT_BATCH];
+    load_choices(p, tb, t1, lane, id);
+#pragma unroll
+    for (int u = 0; u < SORT_BATCH; ++u) {
+      if (id[u] >= 0) cnt[id[u]] += 1;  // a token's experts differ: no two lanes meet
+      __syncwarp();
+    }
+  }
+}
 
 // Sorted place of every pair of this block's tokens.  A token chooses an
 // expert at most once, so the place of a pair within its expert is the number
@@ -72,18 +111,20 @@ __device__ void assign_places(const RouteParams& p, int32_t* s_cnt, const int32_
   }
   __syncthreads();
   int32_t* run = s_cnt + warp * p.Ep;
-  for (int64_t t = t0; t < t1; ++t) {
-    if (lane < p.k) {
-      const int id = p.ids[t * p.k + lane];
+  for (int64_t tb = t0; tb < t1; tb += SORT_BATCH) {
+    int id[SORT_BATCH];
+    load_choices(p, tb, t1, lane, id);
+#pragma unroll
+    for (int u = 0; u < SORT_BATCH; ++u) {
       int at = -1;
-      if (id >= 0) {
-        at = run[id];
-        run[id] = at + 1;
-        p.rows[at] = (int32_t)t;
+      if (id[u] >= 0) {
+        at = run[id[u]];
+        run[id[u]] = at + 1;
+        p.rows[at] = (int32_t)(tb + u);
       }
-      p.pos[t * p.k + lane] = at;
+      if (lane < p.k && tb + u < t1) p.pos[(tb + u) * p.k + lane] = at;
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -117,98 +158,104 @@ __device__ int scan_experts(const RouteParams& p, const int32_t* s_tot, int32_t*
   return *s_total;
 }
 
-// One warp per token: lane l holds logits l, l + 32, ...; k rounds of the
-// warp's maximum (the lowest index where values tie), each two warp-wide
-// reductions, leave slot j's expert and logit in lane j.
-template <int DT, int PER>
+// L lanes a token, PER logits a lane (expert sub + L * i), 32 / L tokens a warp
+// at a time.  k rounds find the largest key below the round's before: PER
+// compares a lane and log2(L) exchanges, for all the warp's tokens at once.
+// (A warp a token with two redux.sync a round took 25 us for 16384 tokens, 128
+// experts and k 8: that instruction issues every 16 clocks or so.)
+template <int DT, int PER, int L>
 __global__ void __launch_bounds__(ROUTE_THREADS) route_topk_kernel(RouteParams p) {
+  using Key = RouteKey<DT>;
+  using KT = typename Key::T;
+  constexpr int TOK = 32 / L;
   extern __shared__ int32_t s_route[];
   int32_t* s_cnt = s_route;                       // [warps][Ep]
   int32_t* s_tot = s_cnt + ROUTE_WARPS * p.Ep;    // [Ep]
   int32_t* s_base = s_tot + p.Ep;                 // [Ep]
+  KT* s_win = reinterpret_cast<KT*>(s_base + p.Ep);  // [warps][TOK][32]: the chosen keys
   __shared__ int32_t s_total;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < ROUTE_WARPS * p.Ep; i += ROUTE_THREADS) s_cnt[i] = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1);
+  for (int i = threadIdx.x; i < (ROUTE_WARPS + 1) * p.Ep; i += ROUTE_THREADS) s_cnt[i] = 0;
   __syncthreads();
   pdl_wait();
   const int64_t per_warp = p.tokens / ROUTE_WARPS;
   const int64_t t0 = min((int64_t)blockIdx.x * p.tokens + warp * per_warp, p.T);
   const int64_t t1 = min(t0 + per_warp, p.T);
   const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.logits);
-  int32_t* cnt = s_cnt + warp * p.Ep;
-  for (int64_t t = t0; t < t1; ++t) {
+  const KT none = Key::make(NEG_INF, 0) | 0xFFFFu;  // no key of -inf is above
+  KT* win = s_win + (warp * TOK + lane / L) * 32;
+  for (int64_t tb = t0; tb < t1; tb += TOK) {
+    const int64_t t = tb + lane / L;
+    const bool in = t < t1;
     float v[PER];
-    uint32_t key[PER];
+    KT key[PER];
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = lane + 32 * i;
-      v[i] = e < p.E ? Elem<DT>::to_f(x[t * p.ld + e]) : NEG_INF;
-      const bool bad = v[i] != v[i];
-      nan |= bad;
-      key[i] = ordered(bad ? NEG_INF : v[i] + 0.0f);  // -0 and +0 tie
+      const int e = sub + L * i;
+      v[i] = in && e < p.E ? Elem<DT>::to_f(x[t * p.ld + e]) : NEG_INF;
+      nan |= v[i] != v[i];
+      key[i] = Key::make(v[i], e);
     }
-    const uint32_t none = ordered(NEG_INF);
-    int my_id = -1;
-    float my_v = NEG_INF;
+    KT last = ~(KT)0;
     for (int j = 0; j < p.k; ++j) {
-      uint32_t best = key[0];
-      int at = 0;
+      KT best = 0;
 #pragma unroll
-      for (int i = 1; i < PER; ++i)
-        if (key[i] > best) { best = key[i]; at = i; }
-      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      if (m <= none) break;  // the rest may not be chosen
-      const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
+      for (int i = 0; i < PER; ++i) {
+        const KT c = key[i] < last ? key[i] : 0;
+        best = c > best ? c : best;
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) {
+        const KT c = __shfl_xor_sync(0xffffffffu, best, o);
+        best = c > best ? c : best;
+      }
+      last = best;
+      if (sub == 0) win[j] = best;
+    }
+    __syncwarp();
+    nan = __any_sync(0xffffffffu >> (32 - L) << (lane & ~(L - 1)), nan);
+    // weights: e / sum; slots sub, sub + L, ... in this lane
+    const bool any = win[0] > none;
+    const float first = Key::value(win[0]);
+    const float top = p.sigmoid ? log_sigmoid(first) : first;
+    float sum = 0.0f;
+    if (!p.sigmoid && !p.renorm) {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if ((uint32_t)(lane + 32 * i) == id) key[i] = 0u;
-      if (lane == j) { my_id = (int)id; my_v = unordered(m); }
+        if (sub + L * i < p.E) sum += expf(v[i] - top);
+    } else if (p.renorm) {
+      // s_j / sum s = softmax of the chosen log-sigmoids: no 0 / 0 far below zero
+      for (int j = sub; j < p.k; j += L)
+        if (win[j] > none) sum += expf((p.sigmoid ? log_sigmoid(Key::value(win[j])) : Key::value(win[j])) - top);
     }
-    const bool chosen = my_id >= 0;
-    float w = 0.0f;
-    if (p.sigmoid) {
-      if (p.renorm) {  // s_j / sum s = softmax of the chosen log-sigmoids: no 0 / 0 far below zero
-        const float l = log_sigmoid(my_v);
-        const float ref = __shfl_sync(0xffffffffu, l, 0);
-        const float e = chosen ? expf(l - ref) : 0.0f;
-        w = e / warp_sum(e);
-      } else {
-        w = 1.0f / (1.0f + expf(-my_v));
-      }
-    } else {
-      const float top = __shfl_sync(0xffffffffu, my_v, 0);
-      const float e = chosen ? expf(my_v - top) : 0.0f;
-      float part = e;
-      if (!p.renorm) {
-        part = 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (lane + 32 * i < p.E) part += expf(v[i] - top);
+    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (in) {
+      for (int j = sub; j < p.k; j += L) {
+        const KT c = win[j];
+        const bool chosen = any && c > none;
+        const float y = Key::value(c);
+        float w = 1.0f / (1.0f + expf(-y));
+        if (!p.sigmoid || p.renorm) w = expf((p.sigmoid ? log_sigmoid(y) : y) - top) / sum;
+        if (nan && !p.sigmoid) w = NAN;
+        p.ids[t * p.k + j] = chosen ? Key::expert(c) : -1;
+        p.weights[t * p.k + j] = chosen ? w : 0.0f;
+        if (chosen) atomicAdd(&s_tot[Key::expert(c)], 1);
       }
-      w = e / warp_sum(part);
-      if (__any_sync(0xffffffffu, nan)) w = NAN;
-    }
-    if (lane < p.k) {
-      p.ids[t * p.k + lane] = my_id;
-      p.weights[t * p.k + lane] = chosen ? w : 0.0f;
-      if (chosen) cnt[my_id] += 1;  // a token's experts differ: no two lanes meet
     }
     __syncwarp();
   }
   __syncthreads();
   pdl_launch_dependents();
-  for (int e = threadIdx.x; e < p.Ep; e += ROUTE_THREADS) {
-    int c = 0;
-#pragma unroll
-    for (int w = 0; w < ROUTE_WARPS; ++w) c += s_cnt[w * p.Ep + e];
-    if (p.blocks > 1) p.counts[(int64_t)blockIdx.x * p.Ep + e] = c;
-    else s_tot[e] = c;
+  if (p.blocks > 1) {
+    for (int e = threadIdx.x; e < p.Ep; e += ROUTE_THREADS) p.counts[(int64_t)blockIdx.x * p.Ep + e] = s_tot[e];
+    return;
   }
-  if (p.blocks > 1) return;
   // one block holds all tokens: it sorts them too
-  __syncthreads();
   const int total = scan_experts(p, s_tot, s_base, &s_total, true);
+  count_choices(p, t0, t1, lane, s_cnt + warp * p.Ep);
+  __syncthreads();
   assign_places(p, s_cnt, s_base, t0, t1, warp, lane);
   for (int64_t i = total + threadIdx.x; i < p.T * p.k; i += ROUTE_THREADS) p.rows[i] = -1;
 }
@@ -231,20 +278,13 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_sort_kernel(RouteParams p
   const int64_t per_warp = p.tokens / ROUTE_WARPS;
   const int64_t t0 = min((int64_t)blockIdx.x * p.tokens + warp * per_warp, p.T);
   const int64_t t1 = min(t0 + per_warp, p.T);
-  int32_t* cnt = s_cnt + warp * p.Ep;
-  for (int64_t t = t0; t < t1; ++t) {
-    if (lane < p.k) {
-      const int id = p.ids[t * p.k + lane];
-      if (id >= 0) cnt[id] += 1;
-    }
-    __syncwarp();
-  }
+  count_choices(p, t0, t1, lane, s_cnt + warp * p.Ep);
   int cols = 1;
   while (cols < p.Ep / 4) cols <<= 1;  // <= 128 for E <= 512
   const int col = threadIdx.x & (cols - 1), slices = ROUTE_THREADS / cols;
   if (col < p.Ep / 4) {
     int4 pre = make_int4(0, 0, 0, 0), tot = make_int4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 8
     for (int b = threadIdx.x / cols; b < p.blocks; b += slices) {
       const int4 c = reinterpret_cast<const int4*>(p.counts + (int64_t)b * p.Ep)[col];
       tot.x += c.x; tot.y += c.y; tot.z += c.z; tot.w += c.w;
@@ -266,23 +306,37 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_sort_kernel(RouteParams p
 }
 
 void route_plan(int64_t T, int64_t& tokens, int64_t& blocks) {
-  tokens = (T + ROUTE_MAX_BLOCKS - 1) / ROUTE_MAX_BLOCKS;
+  tokens = (T + ROUTE_BLOCKS - 1) / ROUTE_BLOCKS;
   tokens = (tokens + ROUTE_WARPS - 1) / ROUTE_WARPS * ROUTE_WARPS;
-  if (tokens < ROUTE_MIN_TOKENS) tokens = ROUTE_MIN_TOKENS;
+  if (tokens == 0) tokens = ROUTE_WARPS;  // (T = 0: no blocks)
   blocks = (T + tokens - 1) / tokens;
 }
 
+template <int DT, int PER, int L>
+int launch_topk_cfg(const RouteParams& p, cudaStream_t s) {
+  const size_t smem = (size_t)(ROUTE_WARPS + 2) * p.Ep * sizeof(int32_t) +
+                      (size_t)ROUTE_WARPS * (32 / L) * 32 * sizeof(typename RouteKey<DT>::T);
+  auto kern = route_topk_kernel<DT, PER, L>;
+  static std::atomic<uint64_t> attr_devices{0};  // shared-memory limit raised once per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  cudaError_t e;
+  if (!(attr_devices.load() & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(route)");
+    attr_devices.fetch_or(bit);
+  }
+  e = launch_pdl(kern, dim3((unsigned)p.blocks), dim3(ROUTE_THREADS), smem, s, p);
+  return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "route launch");
+}
 template <int DT>
 int launch_topk(const RouteParams& p, cudaStream_t s) {
-  const size_t smem = (size_t)(ROUTE_WARPS + 2) * p.Ep * sizeof(int32_t);
-  const dim3 grid((unsigned)p.blocks), block(ROUTE_THREADS);
-  cudaError_t e;
-  if (p.E <= 32) e = launch_pdl(route_topk_kernel<DT, 1>, grid, block, smem, s, p);
-  else if (p.E <= 64) e = launch_pdl(route_topk_kernel<DT, 2>, grid, block, smem, s, p);
-  else if (p.E <= 128) e = launch_pdl(route_topk_kernel<DT, 4>, grid, block, smem, s, p);
-  else if (p.E <= 256) e = launch_pdl(route_topk_kernel<DT, 8>, grid, block, smem, s, p);
-  else e = launch_pdl(route_topk_kernel<DT, 16>, grid, block, smem, s, p);
-  return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "route launch");
+  if (p.E <= 32) return launch_topk_cfg<DT, 4, 8>(p, s);
+  if (p.E <= 64) return launch_topk_cfg<DT, 8, 8>(p, s);
+  if (p.E <= 128) return launch_topk_cfg<DT, 16, 8>(p, s);
+  if (p.E <= 256) return launch_topk_cfg<DT, 16, 16>(p, s);
+  return launch_topk_cfg<DT, 16, 32>(p, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -804,6 +804,7 @@ def test_abi_refusals(pkg):
     n = ctypes.c_uint64(7)
     assert lib.qlin_route_experts_workspace(1, 8, ctypes.addressof(n)) == 0 and n.value == 0
     assert lib.qlin_route_experts_workspace(100000, 9, ctypes.addressof(n)) == 0 and n.value > 0 and n.value % 16 == 0
+    assert lib.qlin_route_experts_workspace(0, 8, ctypes.addressof(n)) == 0 and n.value == 0
     assert lib.qlin_route_experts_workspace(1, 0, ctypes.addressof(n)) == bad
     assert lib.qlin_route_experts_workspace(1, 8, None) == bad
     comb = lambda y=16, R=4, Nn=8, ld=8, T=2, k=2, res=None, ldr=8, dt=N.BF16: lib.qlin_combine_experts(
