@@ -356,55 +356,101 @@ struct CombineParams {
   int64_t chunks;        // blocks a token
 };
 
-// One thread per VEC columns of a token: a float32 sum in slot order, rounded
-// once.  HBM bound: every row of y that a token chose is read once.
-template <int DT, int VEC>
-__global__ void __launch_bounds__(128) combine_kernel(CombineParams p) {
+constexpr int COMBINE_THREADS = 128;
+
+// One thread per CH chunks of VEC columns of a token, COMBINE_THREADS chunks
+// apart: a float32 sum in slot order, rounded once.  HBM bound: every row of y
+// that a token chose is read once; BATCH of them are on their way at a time.
+template <int DT, int VEC, int CH, int BATCH>
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(CombineParams p) {
   using T = typename Elem<DT>::T;
+  union alignas(sizeof(T) * VEC) Chunk {
+    uint4 whole;  // VEC > 1: 16 bytes, moved at once
+    T v[VEC];
+    __device__ Chunk() {}
+    __device__ void load(const void* from) {
+      if constexpr (VEC == 1) v[0] = *static_cast<const T*>(from);
+      else whole = __ldcs(static_cast<const uint4*>(from));  // read once
+    }
+    __device__ void store(void* to) const {
+      if constexpr (VEC == 1) *static_cast<T*>(to) = v[0];
+      else *static_cast<uint4*>(to) = whole;
+    }
+  };
   pdl_wait();
   pdl_launch_dependents();
   const int64_t t = blockIdx.x / p.chunks;
-  const int64_t col = ((blockIdx.x % p.chunks) * 128 + threadIdx.x) * VEC;
-  if (col >= p.N) return;
-  const T* y = reinterpret_cast<const T*>(p.y) + col;
-  float acc[VEC];
+  const int64_t col0 = (blockIdx.x % p.chunks) * (COMBINE_THREADS * CH * VEC) + threadIdx.x * VEC;
+  const auto column = [&](int c) { return col0 + c * (COMBINE_THREADS * VEC); };
+  Chunk res[CH];
+  if (p.residual != nullptr) {  // on its way while the rows are added up
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-  for (int j = 0; j < p.k; ++j) {
-    const int at = p.pos[t * p.k + j];
-    if (at < 0 || at >= p.R) continue;
-    const float w = p.weights[t * p.k + j];
-    alignas(16) T v[VEC];
-    if constexpr (VEC == 1) v[0] = y[at * p.ldy];
-    else *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(y + at * p.ldy));
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = __fmaf_rn(w, Elem<DT>::to_f(v[i]), acc[i]);
+    for (int c = 0; c < CH; ++c)
+      if (column(c) < p.N)
+        res[c].load(reinterpret_cast<const T*>(p.residual) + t * p.ld_res + column(c));
   }
-  alignas(16) T v[VEC];
-  if (p.residual != nullptr) {
-    const T* r = reinterpret_cast<const T*>(p.residual) + t * p.ld_res + col;
-    if constexpr (VEC == 1) v[0] = r[0];
-    else *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(r));
+  float acc[CH][VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] += Elem<DT>::to_f(v[i]);
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
+  for (int j0 = 0; j0 < p.k; j0 += BATCH) {
+    int at[BATCH];
+    float w[BATCH];
+    Chunk v[BATCH][CH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      at[u] = j0 + u < p.k ? __ldg(p.pos + t * p.k + j0 + u) : -1;
+      w[u] = j0 + u < p.k ? __ldg(p.weights + t * p.k + j0 + u) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (at[u] >= 0 && at[u] < p.R) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (column(c) < p.N)
+            v[u][c].load(reinterpret_cast<const T*>(p.y) + at[u] * p.ldy + column(c));
+      }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (at[u] >= 0 && at[u] < p.R) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (column(c) < p.N)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[c][i] = __fmaf_rn(w[u], Elem<DT>::to_f(v[u][c].v[i]), acc[c][i]);
+      }
   }
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = Elem<DT>::from_f(acc[i]);
-  T* o = reinterpret_cast<T*>(p.out) + t * p.N + col;
-  if constexpr (VEC == 1) o[0] = v[0];
-  else *reinterpret_cast<uint4*>(o) = *reinterpret_cast<uint4*>(v);
+  for (int c = 0; c < CH; ++c) {
+    if (column(c) >= p.N) continue;
+    Chunk o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      o.v[i] = Elem<DT>::from_f(p.residual != nullptr ? acc[c][i] + Elem<DT>::to_f(res[c].v[i]) : acc[c][i]);
+    o.store(reinterpret_cast<T*>(p.out) + t * p.N + column(c));
+  }
 }
 
-template <int DT>
-int launch_combine_dt(CombineParams p, bool vec, cudaStream_t s) {
-  constexpr int VEC = 16 / sizeof(typename Elem<DT>::T);
-  const int64_t per = 128 * (vec ? VEC : 1);
+template <int DT, int VEC, int CH, int BATCH>
+int launch_combine_cfg(CombineParams p, cudaStream_t s) {
+  constexpr int64_t per = COMBINE_THREADS * CH * VEC;
   p.chunks = (p.N + per - 1) / per;
   if (p.chunks * p.T > INT32_MAX) return fail(QLIN_ERR_UNSUPPORTED, "combine: too many tokens");
-  const dim3 grid((unsigned)(p.chunks * p.T));
-  const cudaError_t e = vec ? launch_pdl(combine_kernel<DT, VEC>, grid, dim3(128), 0, s, p)
-                            : launch_pdl(combine_kernel<DT, 1>, grid, dim3(128), 0, s, p);
+  const cudaError_t e =
+      launch_pdl(combine_kernel<DT, VEC, CH, BATCH>, dim3((unsigned)(p.chunks * p.T)), dim3(COMBINE_THREADS), 0, s, p);
   return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "combine launch");
+}
+template <int DT>
+int launch_combine_dt(const CombineParams& p, bool vec, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(typename Elem<DT>::T);
+  if (!vec) return launch_combine_cfg<DT, 1, 8, 4>(p, s);
+  // Few rows a token: two chunks a thread, else its loads are too few (4096
+  // tokens of 4096 bf16, k 2 and a residual: 20.6 us, 6.5 TB/s; with one chunk
+  // 27.8).  With more rows a token one chunk has enough (k 8: 50.6 us, with two
+  // 56).
+  if (p.k <= 2) return launch_combine_cfg<DT, VEC, 2, 2>(p, s);
+  return launch_combine_cfg<DT, VEC, 1, 4>(p, s);
 }
 
 }  // namespace
