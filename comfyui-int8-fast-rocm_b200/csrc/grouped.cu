@@ -58,6 +58,7 @@ struct GroupedParams {
   const void* bias;        // [E, N] in the output dtype, or null
   void* out;               // [R, N]
   int R, N, K;
+  int early;               // the kernel before this one is gather_kernel
 };
 
 struct Smem {  // behind the operand ring
@@ -224,7 +225,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = s->tmem_slot;
-  pdl_wait();
+  // gather_kernel waits for the kernels before it, then lets this one start:
+  // only the rows' order (a, a_scale) is still to come, and the weights are on
+  // their way before it
+  if (!p.early) pdl_wait();
   pdl_launch_dependents();
 
   // Row ranges and tile numbers of the experts, whatever the offsets hold.
@@ -247,24 +251,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       uint32_t phase = 0;
       Armed armed;
       bool ok = true;
+      int ahead = 0;  // stages whose weights were asked for before the rows could be
+      auto load_w = [&](int st, const Tile& t, int kb) {
+        const uint32_t fb = mapa_shared(smem_u32(&s->full[st]), 0);
+        if (leader) mbar_arrive_expect_tx(&s->full[st], 2 * SL * (SLAB + (16 << box_of(t)) * BK));
+        const int row = t.e * p.N + t.n0 + (int)rank * BM;
+        if constexpr (SL == 1) tma_load_2d_pair(sW + st * SLAB, &tmW, fb, kb * BK, row);
+        else tma_load_3d_pair(sW + st * SL * SLAB, &tmW, fb, 0, row, kb * SL);
+      };
+      if (p.early) {
+        int ea = 0;
+        for (int tile = first; tile < num_tiles && ahead < STAGES; tile += step) {
+          const Tile t = locate(s, tile, ea);
+          for (int kb = 0; kb < num_kb && ahead < STAGES; ++kb) load_w(ahead++, t, kb);
+        }
+        pdl_wait();
+      }
       for (int tile = first; tile < num_tiles && ok; tile += step) {
         const Tile t = locate(s, tile, e);
-        const int half = t.width >> 1;
-        const int wrow = t.e * p.N + t.n0 + (int)rank * BM, xrow = t.row0 + (int)rank * half;
-        const int box = box_of(t);
-        const CUtensorMap* tmx = &tmX.box[box];
-        const uint32_t bytes = 2 * SL * (SLAB + (16 << box) * BK);
+        const int xrow = t.row0 + (int)rank * (t.width >> 1);
+        const CUtensorMap* tmx = &tmX.box[box_of(t)];
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          if (ahead > 0) --ahead;
+          else load_w(stage, t, kb);
           const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
-          if (leader) mbar_arrive_expect_tx(&s->full[stage], bytes);
-          if constexpr (SL == 1) {
-            tma_load_2d_pair(sW + stage * SLAB, &tmW, fb, kb * BK, wrow);
-            tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
-          } else {
-            tma_load_3d_pair(sW + stage * SL * SLAB, &tmW, fb, 0, wrow, kb * SL);
-            tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
-          }
+          if constexpr (SL == 1) tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
+          else tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
           armed.note(stage, phase);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -316,6 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     using EO = Elem<DT>;
     using T = typename EO::T;
     const int tid = threadIdx.x - 64, quarter = warp & 3, part = (warp - 2) >> 2;
+    if (p.early) pdl_wait();  // before anything is written, or a scale read
     {  // rows of no expert
       const int64_t line = (int64_t)p.N * sizeof(T);
       const int64_t thread = (int64_t)blockIdx.x * 32 * EPI_WARPS + tid, count = (int64_t)gridDim.x * 32 * EPI_WARPS;
@@ -445,7 +459,8 @@ int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8
   for (int i = 0; i < BOXES && !rc; ++i)
     rc = encode_slab_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i, slabs);
   if (rc) return rc;
-  const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K};
+  const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K,
+                        a_rows != nullptr};
   // tiles at most: every expert adds one partly filled row block to R / 256
   const int64_t tiles = (R / BT + (E < R ? E : R)) * ((N + 2 * BM - 1) / (2 * BM));
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);
