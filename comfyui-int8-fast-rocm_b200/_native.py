@@ -69,7 +69,7 @@ SIGNATURES = {
     "qlin_combine_experts": [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _L, _P, _P],
     "qlin_gemm_w8a8_grouped_workspace": [_L, _L, _P],
     "qlin_gemm_w8a8_grouped": [_P, _P, _L, _P, _P, _P, _L, _P, _P, _P, _I, _L, _L, _L, _P, _U64, _P],
-    "qlin_matvec_w4_workspace": [_L, _L, _P],
+    "qlin_matvec_w4_workspace": [_P, _I, _L, _L, _L, _L, _P],
     "qlin_matvec_w4": [_P, _I, _L, _L, _P, _P, _I, _I, _P, _L, _P, _P, _P, _L, _L, _L, _P, _U64, _P],
 }
 

@@ -744,11 +744,13 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
                         workspace, static_cast<cudaStream_t>(stream));
 }
 
-QLIN_API int qlin_matvec_w4_workspace(int64_t Rx, int64_t K, uint64_t* bytes) {
+QLIN_API int qlin_matvec_w4_workspace(const int8_t* w_packed, int has_offsets, int64_t R, int64_t Rx, int64_t N,
+                                      int64_t K, uint64_t* bytes) {
   QLIN_RANGE();
   if (!bytes) return fail(QLIN_ERR_INVALID_ARG, "bytes is null");
-  if (Rx < 0 || K < 0 || Rx > INT32_MAX || K > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "bad shape");
-  *bytes = matvec_workspace_bytes(Rx, K);
+  if (R < 0 || Rx < 0 || N < 0 || K < 0 || R > INT32_MAX || Rx > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+    return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  *bytes = matvec_workspace_bytes(reinterpret_cast<const uint8_t*>(w_packed), has_offsets != 0, R, Rx, N, K);
   return QLIN_OK;
 }
 
@@ -770,9 +772,12 @@ QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx,
     return fail(QLIN_ERR_UNSUPPORTED, "dimension too large");
   if (R == 0 || N == 0) return QLIN_OK;
   if ((Rx > 0 && !x) || !w_packed || !w_scale || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
-  if (Rx > 0 && (!workspace || workspace_bytes < matvec_workspace_bytes(Rx, K)))
-    return fail(QLIN_ERR_INVALID_ARG, "workspace of " + std::to_string(matvec_workspace_bytes(Rx, K)) + " bytes needed");
-  if (!aligned16(workspace)) return fail(QLIN_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  const uint64_t need = matvec_workspace_bytes(reinterpret_cast<const uint8_t*>(w_packed), offsets != nullptr, R, Rx, N,
+                                               K);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(QLIN_ERR_INVALID_ARG, "workspace of " + std::to_string(need) + " bytes needed");
+  if (!aligned16(workspace) || !aligned16(out))
+    return fail(QLIN_ERR_ALIGNMENT, "the output and the workspace must be 16-byte aligned");
   int rc = check_device();
   if (rc) return rc;
   return launch_matvec_w4(x_dtype, x, Rx, ldx, reinterpret_cast<const uint8_t*>(w_packed), w_scale,

@@ -68,6 +68,7 @@ struct MatvecParams {
   int R, N, K;
   int blocks;             // of 128 k
   int early;              // the kernel before this one is split_kernel
+  int own_digits;         // matvec_kernel makes the digits itself (one pass of one expert)
   int tile;               // weight rows a stage: 32 to 256
   int whole;              // a stage is one three-dimensional TMA box (rows are whole slabs of 128 bytes)
   int stages;
@@ -94,56 +95,69 @@ __device__ __forceinline__ int64_t source_row(const MatvecParams& p, int r) {
 // activations -> digits
 // ---------------------------------------------------------------------------
 
-// One block a row, a warp 128 k at a time; lane l has k 4l .. 4l + 3 of them.
+// Lane l of a warp has k 4l .. 4l + 3 of a block of 128.
+template <int DT>
+__device__ __forceinline__ void load_x4(const MatvecParams& p, int64_t src, int b, int lane, float (&v)[4]) {
+  const int k = b * KB + 4 * lane;
+  const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + src * p.ldx + k;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = src >= 0 && k + i < p.K ? Elem<DT>::to_f(x[i]) : 0.0f;
+}
+// The block's digits to out [half][digit][lane t][16 bytes], 2^e to *exp;
+// whether there are infinities or NaN (which add nothing here, see odd_terms).
 // The matrix instruction meets a word of eight nibbles as its even and its
 // odd ones, so the digits of k 0 2 4 6 and of 1 3 5 7 of each eight lie
 // together; lane t of the product reads words 4t .. 4t + 3 of a block, two at
 // a time.
+__device__ __forceinline__ bool make_digits(float (&v)[4], int lane, void* out, float* exp) {
+  uint32_t big = 0;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!(fabsf(v[i]) <= 3.402823466e38f)) {
+      odd = true;
+      v[i] = 0.0f;
+    }
+    big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  }
+  big = __reduce_max_sync(0xffffffffu, big);
+  const int e = max((int)(big >> 23), 1) - 127;  // |x| < 2^(e + 1)
+  // 2^(29 - e) in two factors, each a float
+  const float f1 = pow2((29 - e) >> 1), f2 = pow2(29 - e - ((29 - e) >> 1));
+  uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit q of the four k
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int X = __float2int_rn(__fmul_rn(__fmul_rn(v[i], f1), f2));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      d[q] |= ((uint32_t)X & 0xFFu) << (8 * i);
+      X = (X + 128) >> 8;  // the signed digit taken off
+    }
+  }
+  const int word = lane >> 1;  // of eight k: the even lane stores its even ones, the odd lane its odd ones
+  uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + (word >> 1 & 1) * 256 + (word >> 2) * 16 +
+                                             (word & 1) * 8 + (lane & 1) * 4);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, d[q], 1);
+    to[q * 16] = lane & 1 ? __byte_perm(other, d[q], 0x7531) : __byte_perm(d[q], other, 0x6420);
+  }
+  if (lane == 0) *exp = pow2(e);
+  return __any_sync(0xffffffffu, odd);
+}
+
+// One block a row, a warp 128 k at a time.
 template <int DT>
 __global__ void __launch_bounds__(1024) split_kernel(MatvecParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
   const int64_t r = blockIdx.x;
-  const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + r * p.ldx;
   bool odd = false;
   for (int b = warp; b < p.blocks; b += blockDim.x >> 5) {
-    const int k = b * KB + 4 * lane;
     float v[4];
-    uint32_t big = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = k + i < p.K ? Elem<DT>::to_f(x[k + i]) : 0.0f;
-      if (!(fabsf(v[i]) <= 3.402823466e38f)) {  // added separately, see odd_terms
-        odd = true;
-        v[i] = 0.0f;
-      }
-      big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    }
-    big = __reduce_max_sync(0xffffffffu, big);
-    const int e = max((int)(big >> 23), 1) - 127;  // |x| < 2^(e + 1)
-    // 2^(29 - e) in two factors, each a float
-    const float f1 = pow2((29 - e) >> 1), f2 = pow2(29 - e - ((29 - e) >> 1));
-    uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit q of the four k
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int X = __float2int_rn(__fmul_rn(__fmul_rn(v[i], f1), f2));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int digit = (int)(int8_t)(X & 0xFF);
-        d[q] |= ((uint32_t)digit & 0xFFu) << (8 * i);
-        X = (X - digit) >> 8;
-      }
-    }
-    const int word = lane >> 1;  // of eight k
-    uint8_t* out = reinterpret_cast<uint8_t*>(p.digits) + (r * p.blocks + b) * (4 * KB) + (word >> 1 & 1) * 256 +
-                   (word >> 2) * 16 + (word & 1) * 8 + 2 * (lane & 1);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      *reinterpret_cast<uint16_t*>(out + q * 64) = (uint16_t)__byte_perm(d[q], 0u, 0x4420);      // k 0, 2
-      *reinterpret_cast<uint16_t*>(out + q * 64 + 4) = (uint16_t)__byte_perm(d[q], 0u, 0x4431);  // k 1, 3
-    }
-    if (lane == 0) p.exps[r * p.epitch + b] = pow2(e);
+    load_x4<DT>(p, r, b, lane, v);
+    odd |= make_digits(v, lane, p.digits + (r * p.blocks + b) * (4 * KB), p.exps + r * p.epitch + b);
   }
   if (__syncthreads_or(odd))
     for (int b = threadIdx.x; b < p.blocks; b += blockDim.x) p.exps[r * p.epitch + b] *= -1.0f;
@@ -178,6 +192,7 @@ __device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, 
 struct Smem {  // behind the ring, the digits, the partial sums and the scales
   uint64_t full[MAX_STAGES], empty[MAX_STAGES], pfull[3], pempty[3], xfull, xempty;
   int abort_flag;
+  uint32_t odd;                // own_digits: rows with infinities or NaN
   int begin[MAX_EXPERTS + 1];  // first row of each expert, ascending within [0, R]
   int cum[MAX_EXPERTS + 1];    // passes before each expert's
 };
@@ -261,9 +276,10 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       mbar_init(&s->pfull[i], WARPS);
       mbar_init(&s->pempty[i], 1);
     }
-    mbar_init(&s->xfull, 1);
+    mbar_init(&s->xfull, p.own_digits ? WARPS : 1);
     mbar_init(&s->xempty, WARPS + 1);
     *abort_flag = 0;
+    s->odd = 0u;
     fence_mbar_init();
   }
   pdl_launch_dependents();
@@ -314,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     int now = -1;
     uint32_t loads = 0;
     Item it;
-    for (it.start(p, s); it.left > 0; it.next(p, s)) {
+    for (it.start(p, s); it.left > 0 && !p.own_digits; it.next(p, s)) {
       if (it.pass == now) continue;
       now = it.pass;
       bool ok = true;
@@ -381,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
             const float* q = part + (buf * WARPS + j) * PART + lane * PITCH + r;
             float v = 0.0f;
             for (int k = 0; k < share; ++k) v += q[k * row_groups * PART];
-            if (xexp[r * p.epitch] < 0.0f) v += odd_terms<DT>(p, source_row(p, it.r0 + r), at);
+            if (xexp[r * p.epitch] < 0.0f || s->odd >> r & 1u) v += odd_terms<DT>(p, source_row(p, it.r0 + r), at);
             if constexpr (!GROUPS) v *= rs;
             if (p.bias != nullptr) v += b;
             reinterpret_cast<T*>(p.out)[(int64_t)(it.r0 + r) * p.N + n] = Elem<DT>::from_f(v);
@@ -438,6 +454,26 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       }
     };
     for (int i = 0; i < AHEAD - 1; ++i) fetch();
+    if (p.own_digits) {
+      constexpr int UN = 4;  // blocks whose values are on their way at a time
+      for (int i0 = warp; i0 < p.R * p.blocks; i0 += UN * WARPS) {
+        float v[UN][4];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int i = i0 + u * WARPS, r = i / p.blocks;
+          load_x4<DT>(p, i < p.R * p.blocks ? source_row(p, r) : -1, i - r * p.blocks, lane, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int i = i0 + u * WARPS, r = i / p.blocks;
+          if (i < p.R * p.blocks &&
+              make_digits(v[u], lane, xdig + (int64_t)i * (4 * KB), xexp + r * p.epitch + i - r * p.blocks) && lane == 0)
+            atomicOr(&s->odd, 1u << r);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->xfull);
+    }
     int stage = 0, now = -1, buf = 0, slot = 0;
     uint32_t phase = 0, loads = 0, pphase = 0;
     bool ok = true;
@@ -568,13 +604,16 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
   }
 }
 
-// The same for any K and alignment, digits and weights straight from memory:
-// one warp 16 weight rows and 2 rows of one expert (grid.y: the experts that
-// have rows, one after another).
-template <int DT, bool GROUPS>
+// The same for any K and alignment, digits and weights straight from memory: a
+// block of threads 16 weight rows and 2 * CB rows of one expert at a time (grid.y:
+// the experts that have rows, one after another), each warp every eighth block
+// of K.  A lane reads its 16 bytes of a weight row as the aligned words that
+// hold them, one block ahead.
+template <int DT, int CB, bool GROUPS>
 __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) {
   using T = typename Elem<DT>::T;
   __shared__ int s_begin[MAX_EXPERTS + 1], s_cum[MAX_EXPERTS + 1];
+  __shared__ float s_part[WARPS][16][2 * CB + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
   pdl_launch_dependents();
@@ -595,56 +634,110 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
   if ((int)blockIdx.y >= s_cum[p.E]) return;
   int e = 0;
   while (s_cum[e + 1] <= (int)blockIdx.y) ++e;
-  const int n0 = (blockIdx.x * WARPS + warp) * 16, bytes = p.K >> 1;
-  if (n0 >= p.N) return;
+  const int n0 = blockIdx.x * 16, bytes = p.K >> 1;
   const float unit = (t & 1) ? pow2(16 - 33) : pow2(-33);
-  const int64_t wrow[2] = {(int64_t)e * p.N + min(n0 + g, p.N - 1), (int64_t)e * p.N + min(n0 + 8 + g, p.N - 1)};
-  for (int r0 = s_begin[e]; r0 < s_begin[e + 1]; r0 += 2) {
-    const int rows = min(2, s_begin[e + 1] - r0);
-    const int64_t src = source_row(p, min(r0 + (g >> 2), r0 + rows - 1));  // whose digits this lane reads
-    const int64_t sum_src = source_row(p, min(r0 + (t >> 1), r0 + rows - 1));  // whose sums it gets
-    float sum[2] = {0.0f, 0.0f};
-    for (int b = 0; b < p.blocks; ++b) {
-      int acc[4] = {0, 0, 0, 0};
+  const uint32_t* words[2];  // of the row, and where in the first one it begins and in which it ends
+  int shift[2], last[2];
+  int64_t wrow[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t a[2][2];
-        const int at = b * (KB / 2) + 16 * t + 4 * q;  // byte of the row
+  for (int h = 0; h < 2; ++h) {
+    wrow[h] = (int64_t)e * p.N + min(n0 + 8 * h + g, p.N - 1);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.w + wrow[h] * bytes);
+    words[h] = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+    shift[h] = 8 * (int)(at & 3);
+    last[h] = (int)((at & 3) + bytes - 1) >> 2;
+  }
+  auto load = [&](int b, uint32_t (&u)[2][5]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        const int at = b * (KB / 8) + 4 * t + i;
+        u[h][i] = b < p.blocks && at <= last[h] ? __ldg(words[h] + at) : 0u;  // (behind K the digits are 0)
+      }
+  };
+  for (int r0 = s_begin[e]; r0 < s_begin[e + 1]; r0 += 2 * CB) {
+    const int rows = min(2 * CB, s_begin[e + 1] - r0);
+    int64_t src[CB], sum_src[CB];  // the rows whose digits this lane reads, whose sums it gets
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      src[c] = source_row(p, r0 + min(2 * c + (g >> 2), rows - 1));
+      sum_src[c] = source_row(p, r0 + min(2 * c + (t >> 1), rows - 1));
+    }
+    float sum[CB][2];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) sum[c][0] = sum[c][1] = 0.0f;
+    uint32_t next[2][5];
+    load(warp, next);
+    for (int b = warp; b < p.blocks; b += WARPS) {
+      uint32_t a[4][2][2];  // [word][row half][even, odd k]: 16 times the nibble
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t u = 0u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (at + i < bytes) u |= (uint32_t)p.w[wrow[h] * bytes + at + i] << (8 * i);
-          a[h][0] = (u << 4) & 0xF0F0F0F0u;
-          a[h][1] = u & 0xF0F0F0F0u;
+          const uint32_t w = __funnelshift_r(next[h][q], next[h][q + 1], shift[h]);
+          a[q][h][0] = (w << 4) & 0xF0F0F0F0u;
+          a[q][h][1] = w & 0xF0F0F0F0u;
         }
-        uint2 v = make_uint2(0u, 0u);
-        if (src >= 0)
-          v = *reinterpret_cast<const uint2*>(p.digits + (src * p.blocks + b) * (4 * KB) + (q >> 1) * 256 + (g & 3) * 64 +
-                                              t * 16 + (q & 1) * 8);
-        mma16832(acc, a[0][0], a[1][0], a[0][1], a[1][1], v.x, v.y);
+      load(b + WARPS, next);
+      float ws[2] = {unit, unit};
+      if constexpr (GROUPS) {
+        ws[0] = __fmul_rn(scale_at(p, wrow[0] * p.groups + b), unit);
+        ws[1] = __fmul_rn(scale_at(p, wrow[1] * p.groups + b), unit);
       }
-      const float xs = sum_src >= 0 ? fabsf(p.exps[sum_src * p.epitch + b]) : 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float v = __int2float_rn(acc[2 * h] + 256 * acc[2 * h + 1]);
-        const float ws = GROUPS ? __fmul_rn(scale_at(p, wrow[h] * p.groups + b), unit) : unit;
-        sum[h] = __fmaf_rn(__fmul_rn(v, ws), xs, sum[h]);
+      for (int c = 0; c < CB; ++c) {
+        uint4 d[2];
+        d[0] = d[1] = make_uint4(0u, 0u, 0u, 0u);
+        if (src[c] >= 0) {
+          const int8_t* from = p.digits + (src[c] * p.blocks + b) * (4 * KB) + (g & 3) * 64 + t * 16;
+          d[0] = *reinterpret_cast<const uint4*>(from);
+          d[1] = *reinterpret_cast<const uint4*>(from + 256);
+        }
+        int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint4& v = d[q >> 1];
+          mma16832(acc, a[q][0][0], a[q][1][0], a[q][0][1], a[q][1][1], (q & 1) ? v.z : v.x, (q & 1) ? v.w : v.y);
+        }
+        const float xs = sum_src[c] >= 0 ? fabsf(p.exps[sum_src[c] * p.epitch + b]) : 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float v = __int2float_rn(acc[2 * h] + 256 * acc[2 * h + 1]);
+          sum[c][h] = __fmaf_rn(__fmul_rn(v, ws[h]), xs, sum[c][h]);
+        }
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v = sum[h] + __shfl_xor_sync(0xffffffffu, sum[h], 1);
-      const int n = n0 + 8 * h + g, r = t >> 1;
-      if ((t & 1) || r >= rows || n >= p.N) continue;
-      const int64_t at = (int64_t)e * p.N + n;
-      if (sum_src >= 0 && p.exps[sum_src * p.epitch] < 0.0f) v += odd_terms<DT>(p, sum_src, at);
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float v = sum[c][h] + __shfl_xor_sync(0xffffffffu, sum[c][h], 1);
+        if (!(t & 1)) s_part[warp][8 * h + g][2 * c + (t >> 1)] = v;
+      }
+    __syncthreads();
+    const int n = n0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
+    if (r < rows && n < p.N) {
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) v += s_part[k][threadIdx.x & 15][r];
+      const int64_t at = (int64_t)e * p.N + n, from = source_row(p, r0 + r);
+      if (from >= 0 && p.exps[from * p.epitch] < 0.0f) v += odd_terms<DT>(p, from, at);
       if constexpr (!GROUPS) v *= scale_at(p, at);
       if (p.bias != nullptr) v += Elem<DT>::to_f(reinterpret_cast<const T*>(p.bias)[at]);
       reinterpret_cast<T*>(p.out)[(int64_t)(r0 + r) * p.N + n] = Elem<DT>::from_f(v);
     }
+    __syncthreads();
   }
+}
+
+// Few values and few weights: every block makes the digits itself.  That takes
+// the device up to a microsecond longer (one row, N 4096, K 4096: 8.2 us, with
+// split_kernel 7.4) but saves a launch and a workspace, 6 of 18 us of a call;
+// with more weights the launch pays, since the ring fills meanwhile (N 24576:
+// 16.6 us, with own digits 19.1).
+bool makes_own_digits(bool experts, int64_t R, int64_t N, int64_t K) {
+  return !experts && R <= 8 && R * K <= 8192 && N * K <= (int64_t)32 << 20;
 }
 
 template <int CB>
@@ -698,17 +791,24 @@ int launch_cb(const MatvecParams& p, cudaStream_t stream) {
 template <int DT>
 int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   cudaError_t e;
+  const int64_t per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
+  const bool fast = aligned && per_row <= SMEM - fixed_bytes<4>() - 65536;  // (the latter: K up to about 34,000)
+  p.own_digits = fast && makes_own_digits(p.offsets != nullptr, p.R, p.N, p.K);
+  p.early = !p.own_digits && p.Rx > 0;
   if (p.early) {
     const int threads = 32 * (p.blocks < 32 ? p.blocks : 32);
     e = launch_pdl(split_kernel<DT>, dim3((unsigned)p.Rx), dim3(threads), 0, stream, p);
     if (e != cudaSuccess) return cuda_fail(e, "matvec_w4 split launch");
   }
-  const int64_t per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
-  if (!aligned || per_row > SMEM - fixed_bytes<4>() - 65536) {  // (the latter: K above 34,000)
+  if (!fast) {
     const int64_t slots = p.offsets == nullptr ? 1 : (p.R < p.E ? p.R : p.E);
-    const dim3 grid((unsigned)((p.N + 16 * WARPS - 1) / (16 * WARPS)), (unsigned)slots), block(32 * WARPS);
-    e = p.groups > 1 ? launch_pdl(matvec_any_kernel<DT, true>, grid, block, 0, stream, p)
-                     : launch_pdl(matvec_any_kernel<DT, false>, grid, block, 0, stream, p);
+    const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)slots), block(32 * WARPS);
+#define QLIN_ANY(CB)                                                                             \
+  e = p.groups > 1 ? launch_pdl(matvec_any_kernel<DT, CB, true>, grid, block, 0, stream, p)      \
+                   : launch_pdl(matvec_any_kernel<DT, CB, false>, grid, block, 0, stream, p)
+    if (p.R <= 2 * slots) QLIN_ANY(1);
+    else QLIN_ANY(4);
+#undef QLIN_ANY
     return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
   }
   // rows an expert, on average: how they spread is known on the device only
@@ -717,6 +817,8 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   if (rows <= MVCB2) return launch_cb<DT, 2>(p, stream);
   return launch_cb<DT, 4>(p, stream);
 }
+
+bool aligned_weights(const uint8_t* w, int64_t K) { return K % 32 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0; }
 
 struct Workspace {
   int64_t blocks, epitch;
@@ -733,7 +835,10 @@ Workspace workspace_layout(int64_t Rx, int64_t K) {
 
 }  // namespace
 
-size_t matvec_workspace_bytes(int64_t Rx, int64_t K) { return workspace_layout(Rx, K).bytes; }
+size_t matvec_workspace_bytes(const uint8_t* w, bool experts, int64_t R, int64_t Rx, int64_t N, int64_t K) {
+  if (aligned_weights(w, K) && makes_own_digits(experts, R, N, K)) return 0;
+  return workspace_layout(Rx, K).bytes;
+}
 
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
@@ -757,11 +862,10 @@ int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8
   p.N = (int)N;
   p.K = (int)K;
   p.blocks = (int)l.blocks;
-  p.early = Rx > 0;
   p.digits = static_cast<int8_t*>(workspace);
   p.exps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + l.exps);
   p.epitch = (int)l.epitch;
-  const bool aligned = K % 32 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  const bool aligned = aligned_weights(w, K);
   if (dt == DT_BF16) return launch_dt<DT_BF16>(p, aligned, stream);
   if (dt == DT_F16) return launch_dt<DT_F16>(p, aligned, stream);
   return launch_dt<DT_F32>(p, aligned, stream);

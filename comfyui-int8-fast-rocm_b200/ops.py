@@ -883,11 +883,12 @@ def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     out = x.new_empty((R, Nn))
     if R and Nn:
         need = ctypes.c_uint64(0)
-        N.call("qlin_matvec_w4_workspace", Rx, K, ctypes.addressof(need))
-        ws = x.new_empty((need.value,), dtype=torch.uint8)  # freed (in stream order) with the call
+        N.call("qlin_matvec_w4_workspace", w_packed.data_ptr(), int(offsets is not None), R, Rx, Nn, K,
+               ctypes.addressof(need))
+        ws = x.new_empty((need.value,), dtype=torch.uint8) if need.value else None  # freed (in stream order) with the call
         N.call("qlin_matvec_w4", x.data_ptr(), dt, Rx, max(ldx, K), w_packed.data_ptr(), w_scale.data_ptr(),
                dtype_code(w_scale.dtype), 128 if groups else 0, _ptr(offsets), E, _ptr(x_rows), _ptr(bias),
-               out.data_ptr(), R, Nn, K, ws.data_ptr(), need.value, st)
+               out.data_ptr(), R, Nn, K, _ptr(ws), need.value, st)
     return out
 
 

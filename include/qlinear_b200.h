@@ -483,9 +483,12 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
  * of no expert become 0.  src(r) = x_rows ? x_rows[r] : r; a source row
  * outside [0, Rx) counts as a row of zeros.  Any R works; the weights are read
  * once for each 2 to 8 rows of an expert, so many rows belong to the GEMMs.
- * workspace: qlin_matvec_w4_workspace(Rx, K) bytes of device memory, 16-byte
- * aligned, used within the call only (NULL when Rx is 0). */
-QLIN_API int qlin_matvec_w4_workspace(int64_t Rx, int64_t K, uint64_t* bytes);
+ * workspace: qlin_matvec_w4_workspace bytes of device memory for these
+ * arguments, 16-byte aligned, used within the call only (NULL when that is 0:
+ * small calls without offsets, no rows).  out is 16-byte aligned; K % 32
+ * == 0 and 16-byte aligned weights are read fastest. */
+QLIN_API int qlin_matvec_w4_workspace(const int8_t* w_packed, int has_offsets, int64_t R, int64_t Rx, int64_t N,
+                                      int64_t K, uint64_t* bytes);
 QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx, const int8_t* w_packed,
                             const void* w_scale, int scale_dtype, int group, const int32_t* offsets, int64_t E,
                             const int32_t* x_rows, const void* bias, void* out, int64_t R, int64_t N, int64_t K,

@@ -456,6 +456,23 @@ def test_matvec_layouts(pkg):
 
 
 @on_gpu
+@pytest.mark.parametrize("K", [256, 130])  # both kernels
+def test_matvec_non_finite_in_few_rows(pkg, K):
+    x, p, s, b = matvec_inputs(23, 2, None, 70, K, False, "f32", True)
+    x[0, 3], x[1, 5] = -math.inf, 2.0
+    for rows in (None, torch.tensor([0, 1], dtype=torch.int32), torch.tensor([1, 0, 1, 0, 0], dtype=torch.int32)):
+        got = run_matvec(pkg, x, p, s, b, None, rows).cpu()
+        y, mag = matvec_ref(x, p, s, b, None, rows)
+        for r, src in enumerate([0, 1] if rows is None else rows.tolist()):
+            if src == 1:
+                assert_matvec(got[r:r + 1], y[r:r + 1], mag[r:r + 1], K)
+            else:
+                q = unpack(p)[:, 3]
+                assert torch.equal(got[r].isnan(), q == 0) and (got[r][q > 0] == -math.inf).all()
+                assert (got[r][q < 0] == math.inf).all()
+
+
+@on_gpu
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_matvec_non_finite_and_large(pkg, dt):
     """Infinities and NaN of a row stay in that row, and so do values near
@@ -821,13 +838,16 @@ def test_abi_refusals(pkg):
     assert lib.qlin_gemm_w8a8_grouped_workspace(-1, 32, ctypes.addressof(n)) == bad
     assert grp(rows=16) == grp(rows=16, ws=16, nws=n.value - 16) == bad
     assert grp(rows=16, ws=8, nws=4096) == align
-    mv = lambda Rx=4, ld=256, sdt=N.F32, group=128, off=None, E=1, R=4, Nn=8, K=256, dt=N.BF16, x=16, ws=16, nws=2 ** 20: lib.qlin_matvec_w4(
-        x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, 16, R, Nn, K, ws, nws, None)
+    mv = lambda Rx=4, ld=256, sdt=N.F32, group=128, off=None, E=1, R=4, Nn=8, K=256, dt=N.BF16, x=16, ws=16, nws=2 ** 20, out=16: lib.qlin_matvec_w4(
+        x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, out, R, Nn, K, ws, nws, None)
     assert mv(E=2) == mv(E=513, off=16) == mv(R=3) == mv(K=255) == mv(ld=255) == mv(sdt=N.F16) == mv(dt=N.I8) == bad
     assert mv(K=250, ld=250) == mv(x=None) == bad
     assert mv(group=64) == unsup
     assert mv(R=0, Rx=0) == mv(Nn=0) == 0
-    assert lib.qlin_matvec_w4_workspace(4, 256, ctypes.addressof(n)) == 0 and n.value >= 4 * 256 * 4
-    assert lib.qlin_matvec_w4_workspace(-1, 256, ctypes.addressof(n)) == bad
-    assert mv(ws=None) == mv(nws=n.value - 1) == bad
-    assert mv(ws=24) == align
+    assert lib.qlin_matvec_w4_workspace(16, 0, 40, 40, 8, 256, ctypes.addressof(n)) == 0 and n.value >= 40 * 256 * 4
+    assert mv(R=40, Rx=40, ws=None) == mv(R=40, Rx=40, nws=n.value - 1) == bad
+    assert mv(ws=24) == mv(out=24) == align
+    assert lib.qlin_matvec_w4_workspace(16, 0, -1, 4, 8, 256, ctypes.addressof(n)) == bad
+    assert lib.qlin_matvec_w4_workspace(16, 0, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value == 0
+    assert lib.qlin_matvec_w4_workspace(17, 0, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value > 0
+    assert lib.qlin_matvec_w4_workspace(16, 1, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value > 0
