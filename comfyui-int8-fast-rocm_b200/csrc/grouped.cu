@@ -13,17 +13,30 @@
 // ragged end of each expert wastes less than 32 columns of one tile instead
 // of up to 255 rows.
 //
-//   warp 0      producer: 128 bytes of K a stage of this CTA's 128 weight rows
-//               and of its half of the tile's rows, one TMA box each, into a
-//               6-stage ring
+//   warp 0      producer: this CTA's 128 weight rows and its half of the tile's
+//               rows, one TMA box each a stage, into a ring of 3 stages of 256
+//               bytes of K (6 of 128 where K is no multiple of 128)
 //   warp 1      TMEM and the pair's MMA issuer (leader CTA)
-//   warps 2-17  epilogue: lane = weight row, column = row of the expert
+//   warps 2-9   epilogue: lane = weight row, column = row of the expert
 //
-// Gathered rows are copied into their order first (gather_kernel): a TMA
-// instruction costs the producer about the same whatever it moves, and at 9
-// or 33 of them a stage (16-row boxes, tile::gather4) they bound the kernel:
-// 8192 rows, 8 experts, N 12288, K 4096: 341 us with boxes of 64 and 16 rows,
-// 432 us with 16, 927 us with gather4, the copy costs 14.
+// What bounds it: with many rows the feed of the tensor cores.  8192 rows, 8
+// experts, N 12288, K 4096 take 289-311 us on different GPUs (2.65-2.85
+// POP/s); one expert of 8192 rows takes 260-275, where the dense GEMM takes
+// 261-270.  Weights that are read for the first time cost 9% of that, the
+// epilogue's stores 8% (a copy of the kernel without each); at K 1536 the
+// stores cost a fifth.  With few rows the weights' bytes: 24 experts with
+// rows, N 2048, K 4096, 202 MB in 39 us (5.1 TB/s), 41.6 with gathered rows.
+//
+// A TMA instruction costs the producer about the same whatever it moves, so
+// each operand comes in one box a stage (the case of 8192 rows: 290 us with
+// 256-byte stages, 301 with 128, 341 with rows in boxes of 64 and 16, 432 in
+// boxes of 16), and gathered rows are copied into their order first
+// (gather_kernel: no measurable cost there; by tile::gather4 927 us).
+//
+// Tried and not kept: L2 prefetches of the weights (297 us), row blocks of
+// equal widths (no change: the pairs share what bounds them), two
+// neighbouring columns a thread through tcgen05.ld.16x256b instead of lane
+// exchanges (K 1536: 3% slower, its stores are half as long).
 //
 // Every wait is bounded; on a timeout the kernel sets the error word, waits
 // for its copies in flight, releases TMEM and returns.
@@ -41,11 +54,8 @@ constexpr int BT = 256;         // rows of an expert a tile at most
 constexpr int BOXES = 4;        // the activations' TMA boxes: 16, 32, 64 and 128 rows
 constexpr int MAX_STAGES = 6;
 constexpr int SLAB = BM * BK;   // 16 KB: a stage of either operand in one CTA
-#ifndef EPIW
-#define EPIW 8
-#endif
-constexpr int EPI_WARPS = EPIW;     // four a quarter of the TMEM lanes: latencies overlap between them
-constexpr int CHUNK = 16;         // columns an epilogue warp takes at a time
+constexpr int EPI_WARPS = 8;    // two a quarter of the TMEM lanes (12 and 16 measured no gain)
+constexpr int CHUNK = 16;       // columns an epilogue warp takes at a time (32: 3% slower at K 1536)
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr int MAX_EXPERTS = QLIN_MAX_EXPERTS;
 constexpr uint32_t TMEM_COLS = 512;  // two accumulators of 256 columns

@@ -22,6 +22,10 @@
 //                  128 are exact; digits and scales meet once a block in
 //                  float32.
 //
+// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 16.6 us: about 6 us
+// of launches and latency, then 5 TB/s; N 98304 4.7 TB/s in all.  From 8 rows
+// on the matrix instructions do: 32 columns of digits, 29.5 us at N 24576.
+//
 // matvec_kernel is persistent, a block of threads a SM.  One warp brings the
 // weights by TMA, 32 or 16 KB a stage of 32 rows or more (loads of 64 bytes a
 // row straight into the lanes that need them stayed at 2 TB/s).  One brings an
@@ -36,9 +40,6 @@
 namespace qlin {
 namespace {
 
-#ifndef MVCB2
-#define MVCB2 4
-#endif
 constexpr int KB = 128;                // k of a block: one weight scale, one exponent
 constexpr int WARPS = 8;               // that multiply
 constexpr int THREADS = 32 * (WARPS + 3);
@@ -811,10 +812,14 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
 #undef QLIN_ANY
     return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
   }
-  // rows an expert, on average: how they spread is known on the device only
+  // Rows a pass by the rows an expert has on average (how they spread is known
+  // on the device only): more columns than rows cost more than a second pass
+  // over an expert's weights, which L2 then holds (32 rows of 8 experts, N
+  // 8192, K 4096: 51 us with 4 rows a pass, 59 with 8; 4 rows of one weight, N
+  // 24576: 20 and 28).
   const int64_t rows = p.offsets == nullptr ? p.R : (p.R < p.E ? 1 : p.R / p.E);
   if (rows <= 2) return launch_cb<DT, 1>(p, stream);
-  if (rows <= MVCB2) return launch_cb<DT, 2>(p, stream);
+  if (rows <= 4) return launch_cb<DT, 2>(p, stream);
   return launch_cb<DT, 4>(p, stream);
 }
 

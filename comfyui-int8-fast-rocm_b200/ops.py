@@ -686,6 +686,8 @@ def _int32(t: torch.Tensor, numel, what: str, device) -> torch.Tensor:
     if t.dtype != torch.int32:
         if t.dtype not in (torch.int64, torch.int16, torch.uint8, torch.int8):
             raise TypeError(f"{what} must hold integers, got {t.dtype}")
+        if t.dtype == torch.int64:  # out of range stays out of range
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         t = t.to(torch.int32)
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{what} must have {numel} entries, got {t.numel()}")

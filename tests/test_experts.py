@@ -318,6 +318,17 @@ def test_grouped_gather_outside_is_zero(pkg):
 
 
 @on_gpu
+def test_indices_beyond_int32_stay_outside(pkg):
+    a, xs, w, ws, _ = grouped_inputs(17, 4, 1, 32, 64, "f32", False)
+    rows = torch.tensor([2 ** 32 + 1, -2 ** 32 + 1, 1], dtype=torch.int64).cuda()
+    off = torch.tensor([0, 2 ** 33], dtype=torch.int64).cuda()
+    y = pkg.ops.gemm_w8a8_grouped(a.cuda(), xs.cuda(), w.cuda(), ws.cuda(), off, rows, None, torch.float32)
+    assert (y[:2] == 0).all() and (y[2] != 0).any()
+    c = pkg.ops.combine_experts(y, torch.ones(1, 2, device="cuda"), torch.tensor([[2, 2 ** 32]]).cuda())
+    assert torch.equal(c[0], y[2])
+
+
+@on_gpu
 def test_grouped_extreme_codes_and_depth(pkg):
     # 128 * 128 * 131056 = 2^31 - 2^18: the largest sum the depth limit lets through
     a, xs, w, ws, _ = grouped_inputs(14, 3, 2, 33, 131056, "f32", False, extreme=True)
@@ -453,6 +464,27 @@ def test_matvec_layouts(pkg):
         got = pkg.ops.matvec_w4(x.cuda(), p.cuda(), buf[at:at + 150].view(50, 3), b.cuda())
         assert_matvec(got, *matvec_ref(x, p, half, b, None, None), 384)
     assert pkg.ops.matvec_w4(x[:0].cuda(), p.cuda(), s.cuda(), b.cuda()).shape == (0, 50)
+
+
+@on_gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("M", [1, 3, 12])
+def test_matvec_large_value_under_a_zero_weight(pkg, dt, M):
+    """A value far above the others of its 128 k sets their unit, 2^-30 of it,
+    also where its own weight is 0: half a unit of each of the 128 at most."""
+    x, p, s, _ = matvec_inputs(24, M, None, 60, 384, True, dt, False)
+    big = 2.0 ** 14
+    x[:, 130] = big
+    p[:, 65] &= -16  # the low nibble of k 130
+    got = run_matvec(pkg, x, p, s, None)
+    y, mag = matvec_ref(x, p, s, None, None, None)
+    off = 2.0 ** -31 * 2 * big * (unpack(p)[:, 128:256].abs().sum(1) * s[:, 1].double())  # (e: below the next power of two)
+    assert ((got.cpu().double() - y).abs() <= off + (384 / 16 + 3 + 40) * 2.0 ** -22 * mag
+            + torch.finfo(TDT[dt]).eps / 2 * 1.001 * y.abs()).all()
+    if dt == "bf16":  # exact down to 2^-22 of the largest: nothing is lost here but the usual
+        near = x.abs() >= big * 2.0 ** -22
+        x = torch.where(near, x, torch.zeros((), dtype=x.dtype))
+        assert_matvec(run_matvec(pkg, x, p, s, None), *matvec_ref(x, p, s, None, None, None), 384)
 
 
 @on_gpu
