@@ -768,7 +768,8 @@ QLIN_API int qlin_matvec_w4(const void* x, int x_dtype, int64_t Rx, int64_t ldx,
     return fail(QLIN_ERR_INVALID_ARG, "scale_dtype must be F32 or BF16");
   if (group != 0 && group != 128) return fail(QLIN_ERR_UNSUPPORTED, "int4 group must be 0 (per row) or 128");
   if (group == 128 && K % 128) return fail(QLIN_ERR_INVALID_ARG, "K must be a multiple of 128 for group-128 int4");
-  if (R > INT32_MAX - 256 || Rx > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 256)
+  if (R > INT32_MAX - 256 || Rx > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 256 ||
+      E * N > INT32_MAX - 256)
     return fail(QLIN_ERR_UNSUPPORTED, "dimension too large");
   if (R == 0 || N == 0) return QLIN_OK;
   if ((Rx > 0 && !x) || !w_packed || !w_scale || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");

@@ -32,6 +32,7 @@
 // expert's activation digits, which stay in shared memory for all its row
 // tiles.  Eight warps multiply, each 32 rows and one or two blocks of 128 k of
 // a stage.  One adds their sums up, in a fixed order, while they go on.
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/qlinear_b200.h"
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
         for (int k = 0; k < BLK; ++k) {
           const int b = b0 + k;
           if (b >= p.blocks) break;
-          float ws[2][2] = {{unit, unit}, {unit, unit}};
+          float ws[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};
           if constexpr (GROUPS) {
             const uint4 u = *reinterpret_cast<const uint4*>(&scales[slot][warp][k][lane & ~3]);
             const uint32_t word[4] = {u.x, u.y, u.z, u.w};
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
             for (int j = 0; j < 4; ++j) {
               float f = __uint_as_float(word[j]);
               if (p.scale_bf16) f = __uint_as_float((upper >> j ^ b) & 1u ? word[j] & 0xFFFF0000u : word[j] << 16);
-              ws[j >> 1][j & 1] = __fmul_rn(f, unit);
+              ws[j >> 1][j & 1] = f;
             }
           }
           const uint8_t* d = ring + stage * STAGE + woff[k];
@@ -575,9 +576,10 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                // |digit sums| <= 128 * 128 * 128: both digits fit an int
-                const float v = __int2float_rn(acc[i][c][2 * h] + 256 * acc[i][c][2 * h + 1]);
-                sum[i][c][h] = __fmaf_rn(__fmul_rn(v, ws[i][h]), xs, sum[i][c][h]);
+                // |digit sums| <= 128 * 128 * 128: both digits fit an int (the
+                // unit goes to the sum, where it is exact however small the scale)
+                const float v = __fmul_rn(__int2float_rn(acc[i][c][2 * h] + 256 * acc[i][c][2 * h + 1]), unit);
+                sum[i][c][h] = __fmaf_rn(GROUPS ? __fmul_rn(v, ws[i][h]) : v, xs, sum[i][c][h]);
               }
           }
         }
@@ -681,10 +683,10 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
           a[q][h][1] = w & 0xF0F0F0F0u;
         }
       load(b + WARPS, next);
-      float ws[2] = {unit, unit};
+      float ws[2] = {1.0f, 1.0f};
       if constexpr (GROUPS) {
-        ws[0] = __fmul_rn(scale_at(p, wrow[0] * p.groups + b), unit);
-        ws[1] = __fmul_rn(scale_at(p, wrow[1] * p.groups + b), unit);
+        ws[0] = scale_at(p, wrow[0] * p.groups + b);
+        ws[1] = scale_at(p, wrow[1] * p.groups + b);
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
@@ -704,8 +706,8 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
         const float xs = sum_src[c] >= 0 ? fabsf(p.exps[sum_src[c] * p.epitch + b]) : 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = __int2float_rn(acc[2 * h] + 256 * acc[2 * h + 1]);
-          sum[c][h] = __fmaf_rn(__fmul_rn(v, ws[h]), xs, sum[c][h]);
+          const float v = __fmul_rn(__int2float_rn(acc[2 * h] + 256 * acc[2 * h + 1]), unit);
+          sum[c][h] = __fmaf_rn(GROUPS ? __fmul_rn(v, ws[h]) : v, xs, sum[c][h]);
         }
       }
     }
@@ -745,6 +747,9 @@ template <int CB>
 constexpr int fixed_bytes() {
   return 1024 + kParts<CB> * WARPS * 32 * (2 * CB + 1) * 4 + AHEAD * WARPS * (kStage<CB> / 16384) * 128 + (int)sizeof(Smem);
 }
+// Bytes of a pass's digits and exponents that every instance has room for, beside 64 KB of weights.
+constexpr int64_t kDigitRoom =
+    SMEM - 65536 - std::max({fixed_bytes<1>(), fixed_bytes<2>(), fixed_bytes<4>()});
 
 template <int DT, int CB, bool GROUPS>
 int launch_cfg(MatvecParams p, cudaStream_t stream) {
@@ -793,7 +798,7 @@ template <int DT>
 int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   cudaError_t e;
   const int64_t per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
-  const bool fast = aligned && per_row <= SMEM - fixed_bytes<4>() - 65536;  // (the latter: K up to about 34,000)
+  const bool fast = aligned && per_row <= kDigitRoom;  // (the latter: K up to about 32,000)
   p.own_digits = fast && makes_own_digits(p.offsets != nullptr, p.R, p.N, p.K);
   p.early = !p.own_digits && p.Rx > 0;
   if (p.early) {

@@ -833,10 +833,11 @@ def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=Non
 def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     """Linear of few rows with packed 4-bit weights, the activations not
     quantised: ``y = dt(x @ (q * scale).T + bias)`` with exact sums of each
-    128 k, float32 sums of those, and one rounding (see qlin_matvec_w4).  ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in
-    place), ``w_packed`` [N, K/2] and ``w_scale`` [N] (or [N, 1]) or
-    [N, K/128], float32 or bfloat16, as :func:`quant_weight_int4` returns
-    them; ``bias`` [N]; the result is in x.dtype.
+    128 k, float32 sums of those, and one rounding (see qlin_matvec_w4).
+    ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in place),
+    ``w_packed`` [N, K/2] and ``w_scale`` [N] (or [N, 1]) or [N, K/128],
+    float32 or bfloat16, as :func:`quant_weight_int4` returns them; ``bias``
+    [N]; the result is in x.dtype.
 
     With ``offsets`` (int32 [E + 1] on the device) the rows are sorted by
     expert: ``w_packed`` [E, N, K/2], ``w_scale`` [E, N] or [E, N, K/128],

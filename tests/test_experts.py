@@ -401,6 +401,25 @@ def test_matvec(pkg, dt, M, Nn, K, groups, bias):
 
 
 @on_gpu
+@pytest.mark.parametrize("K", [32000, 32256, 33024, 33408, 34048])
+@pytest.mark.parametrize("M", [1, 3, 8])
+def test_matvec_depth_at_the_limit_of_shared_memory(pkg, K, M):
+    x, p, s, b = matvec_inputs(K, M, None, 40, K, True, "bf16", True)
+    assert_matvec(run_matvec(pkg, x, p, s, b), *matvec_ref(x, p, s, b, None, None), K)
+
+
+@on_gpu
+@pytest.mark.parametrize("K", [256, 258])  # both kernels (258: one scale a row)
+@pytest.mark.parametrize("xe,se", [(100, -120), (-110, 100), (0, -126), (127, -126)])
+def test_matvec_scales_far_from_one(pkg, K, xe, se):
+    x, p, s, _ = matvec_inputs(25, 3, None, 50, K, K == 256, "f32", False)
+    x = torch.ldexp(x / x.abs().max() * 2.0 ** -8, torch.tensor(xe))
+    s = torch.ldexp(s / s.max(), torch.tensor(se))
+    s = s.clamp_min(torch.finfo(torch.float32).smallest_normal)
+    assert_matvec(run_matvec(pkg, x, p, s, None), *matvec_ref(x, p, s, None, None, None), K)
+
+
+@on_gpu
 @pytest.mark.parametrize("dt,sdt", [("bf16", torch.bfloat16), ("f16", torch.float32), ("f32", torch.bfloat16)])
 @pytest.mark.parametrize("counts,Nn,K,groups", [
     ([1], 40, 128, True), ([0, 3, 0, 1], 65, 256, True), ([2, 9, 40, 1], 24, 384, True), ([1] * 20, 128, 96, False),
@@ -874,7 +893,7 @@ def test_abi_refusals(pkg):
         x, dt, Rx, ld, 16, 16, sdt, group, off, E, None, None, out, R, Nn, K, ws, nws, None)
     assert mv(E=2) == mv(E=513, off=16) == mv(R=3) == mv(K=255) == mv(ld=255) == mv(sdt=N.F16) == mv(dt=N.I8) == bad
     assert mv(K=250, ld=250) == mv(x=None) == bad
-    assert mv(group=64) == unsup
+    assert mv(group=64) == mv(E=512, off=16, Nn=2 ** 23) == unsup
     assert mv(R=0, Rx=0) == mv(Nn=0) == 0
     assert lib.qlin_matvec_w4_workspace(16, 0, 40, 40, 8, 256, ctypes.addressof(n)) == 0 and n.value >= 40 * 256 * 4
     assert mv(R=40, Rx=40, ws=None) == mv(R=40, Rx=40, nws=n.value - 1) == bad
