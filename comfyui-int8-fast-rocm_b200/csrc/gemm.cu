@@ -296,12 +296,6 @@ int encode_slab_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint6
                          {slab_bytes, box_rows, slabs});
 }
 
-int encode_row_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
-                    uint32_t box_rows, uint32_t slabs) {
-  return make_tmap_slabs(m, base, {slab_bytes, row_bytes / slab_bytes, rows}, {slab_bytes, row_bytes},
-                         {slab_bytes, slabs, box_rows});
-}
-
 int launch_gemm(int kind, bool b_int4, const int8_t* a, const int8_t* b, const float* a_scale,
                 const float* w_scale, const void* bias, void* out, int out_dt, int64_t M, int64_t N, int64_t K,
                 cudaStream_t stream) {

@@ -75,6 +75,7 @@ struct Smem {  // behind the operand ring
   uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], drain;
   uint32_t tmem_slot;
   int abort_flag;
+  int ready[2];                      // whether an accumulator was complete in time: what all epilogue threads go by
   alignas(16) float xs[2][BT];       // activation scales of a tile's rows
   int begin[MAX_EXPERTS + 1];        // first row of each expert, ascending within [0, R]
   int cum[MAX_EXPERTS + 1];          // tiles before each expert's
@@ -371,9 +372,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const float wscale = ws, b = bias;
       if (tid < BT) s->xs[acc][tid] = xs;
       // one thread polls; the others sleep at the barrier
-      if (tid == 0) wait_bounded(&s->tfull[acc], acc_phase, abort_flag);
+      if (tid == 0) s->ready[acc] = wait_bounded(&s->tfull[acc], acc_phase, abort_flag);
       epilogue_barrier();
-      if (*abort_flag) break;
+      if (!s->ready[acc]) break;
       tc_fence_after();
       if (tile + step < num_tiles) fetch(tile + step);
       for (int c = part * CHUNK; c < now.rows; c += EPI_WARPS / 4 * CHUNK) {

@@ -165,10 +165,6 @@ int launch_situ(int dt, const void* x, int64_t ldx, int64_t M, int64_t K, void* 
 // boxes of that many slabs behind each other (gemm.cu).
 int encode_slab_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
                      uint32_t box_rows, uint32_t slabs);
-// The same rows as {byte in slab, slab, row}: boxes of box_rows rows of
-// `slabs` slabs each, a row's slabs behind each other.
-int encode_row_tmap(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t slab_bytes,
-                    uint32_t box_rows, uint32_t slabs);
 
 // Mixture-of-experts operators (experts.cu, grouped.cu, matvec.cu).
 size_t route_workspace_bytes(int64_t T, int64_t E);
