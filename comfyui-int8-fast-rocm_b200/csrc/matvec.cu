@@ -195,6 +195,7 @@ struct Smem {  // behind the ring, the digits, the partial sums and the scales
   uint64_t full[MAX_STAGES], empty[MAX_STAGES], pfull[3], pempty[3], xfull, xempty;
   int abort_flag;
   uint32_t odd;                // own_digits: rows with infinities or NaN
+  int first_items, first_pass, first_n0;  // this block of threads' items: how many, and where they begin
   int begin[MAX_EXPERTS + 1];  // first row of each expert, ascending within [0, R]
   int cum[MAX_EXPERTS + 1];    // passes before each expert's
 };
@@ -211,13 +212,19 @@ struct Item {
     r0 = s->begin[e] + r;
     rows = min(p.pass, s->begin[e + 1] - r0);
   }
+  // Once a block of threads: the divisions took each warp a microsecond.
+  static __device__ __forceinline__ void share_out(const MatvecParams& p, Smem* s) {
+    const uint32_t tiles = (uint32_t)(p.N + p.tile - 1) / (uint32_t)p.tile, items = (uint32_t)s->cum[p.E] * tiles;
+    const uint32_t each = items / gridDim.x, more = items - each * gridDim.x;  // (items fit an int: see launch_cfg)
+    const uint32_t first = blockIdx.x * each + min(blockIdx.x, more), pass = first / tiles;
+    s->first_items = (int)(each + (blockIdx.x < more));
+    s->first_pass = (int)pass;
+    s->first_n0 = (int)(first - pass * tiles) * p.tile;
+  }
   __device__ __forceinline__ void start(const MatvecParams& p, const Smem* s) {
-    const int tiles = (p.N + p.tile - 1) / p.tile;
-    const int64_t items = (int64_t)s->cum[p.E] * tiles;
-    const int first = (int)(items * blockIdx.x / gridDim.x);
-    left = (int)(items * (blockIdx.x + 1) / gridDim.x) - first;
-    pass = first / tiles;
-    n0 = (first - pass * tiles) * p.tile;
+    left = s->first_items;
+    pass = s->first_pass;
+    n0 = s->first_n0;
     e = 0;
     if (left > 0) find(p, s);
   }
@@ -292,7 +299,11 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     s->begin[threadIdx.x] = threadIdx.x ? p.R : 0;
   }
   __syncthreads();
-  if (warp == 0) expert_bounds(s->begin, s->cum, p.E, lane, [&](int rows) { return (rows + p.pass - 1) / p.pass; });
+  if (warp == 0) {
+    expert_bounds(s->begin, s->cum, p.E, lane, [&](int rows) { return (rows + p.pass - 1) / p.pass; });
+    __syncwarp();
+    if (lane == 0) Item::share_out(p, s);
+  }
   __syncthreads();
   const int slabs = STAGE / (128 * p.tile);                    // of 128 bytes a row and stage
   const int steps = (p.blocks + 2 * slabs - 1) / (2 * slabs);  // stages of a tile
@@ -521,8 +532,10 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
         if (!wait_bounded(&s->full[stage], phase, abort_flag)) { ok = false; break; }
 #pragma unroll
         for (int k = 0; k < BLK; ++k) {
-          const int b = b0 + k;
-          if (b >= p.blocks) break;
+          // Behind K the weights are 0, and the last block's digits and exponent
+          // serve; a branch here would keep the two blocks of a warp one behind
+          // the other.
+          const int b = min(b0 + k, p.blocks - 1);
           float ws[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};
           if constexpr (GROUPS) {
             const uint4 u = *reinterpret_cast<const uint4*>(&scales[slot][warp][k][lane & ~3]);
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
             for (int j = 0; j < 4; ++j) {
               float f = __uint_as_float(word[j]);
               if (p.scale_bf16) f = __uint_as_float((upper >> j ^ b) & 1u ? word[j] & 0xFFFF0000u : word[j] << 16);
-              ws[j >> 1][j & 1] = f;
+              ws[j >> 1][j & 1] = b0 + k < p.blocks ? f : 0.0f;
             }
           }
           const uint8_t* d = ring + stage * STAGE + woff[k];
