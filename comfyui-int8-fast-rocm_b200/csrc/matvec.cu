@@ -43,7 +43,7 @@ namespace {
 
 constexpr int KB = 128;                // k of a block: one weight scale, one exponent
 constexpr int WARPS = 8;               // that multiply
-constexpr int THREADS = 32 * (WARPS + 3);
+constexpr int THREADS = 32 * (WARPS + 4);
 // Bytes of weights a stage, 2 or 1 blocks of 128 k a warp: with few columns
 // the larger, whose fixed costs are half (the digits of eight rows leave no
 // room for it).
@@ -51,7 +51,9 @@ template <int CB> constexpr int kStage = CB <= 2 ? 32768 : 16384;
 // Buffers of partial sums between the multiplying warps and the one that adds them up.
 template <int CB> constexpr int kParts = CB <= 2 ? 3 : 2;
 constexpr int MAX_STAGES = 12;
-constexpr int AHEAD = 8;               // stages a multiplying warp's weight scales are read ahead, less one
+// Room for a stage's weight scales, see scale_pitch.
+template <int CB> constexpr int kScales = kStage<CB> / 32 * 3;
+enum Scales { ROW, GROUP_F32, GROUP_BF16 };  // one a row (in the epilogue), or a row and block of 128 k
 constexpr int MAX_EXPERTS = QLIN_MAX_EXPERTS;
 constexpr int SMEM = 227 * 1024;
 
@@ -72,6 +74,7 @@ struct MatvecParams {
   int early;              // the kernel before this one is split_kernel
   int own_digits;         // matvec_kernel makes the digits itself (one pass of one expert)
   int tile;               // weight rows a stage: 32 to 256
+  int scale_copy;         // bytes of a copy of weight scales: 16, 8 or 4, 2 for plain loads
   int whole;              // a stage is one three-dimensional TMA box (rows are whole slabs of 128 bytes)
   int stages;
   int pass;               // rows of an expert whose digits fit, at most 2 * CB
@@ -239,14 +242,20 @@ struct Item {
   }
 };
 
-__device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// The barrier counts this thread once its copies are complete.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Bytes from one row's weight scales of a stage to the next row's: the eight
+// rows that a warp reads at once lie in different banks.  tile * pitch is at
+// most 3072 with 32 KB of weights a stage, half of that with 16.
+__host__ __device__ constexpr int scale_pitch(int bytes) { return bytes > 16 ? bytes + 16 : bytes; }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
   asm volatile(
@@ -259,7 +268,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_
 // Everything read before pdl_wait was complete before split_kernel let this
 // kernel start (it waits for the kernels before it first).
 // CB: blocks of 8 columns, two rows each.
-template <int DT, int CB, bool GROUPS>
+template <int DT, int CB, Scales SC>
 __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constant__ CUtensorMap tmW, MatvecParams p) {
   using T = typename Elem<DT>::T;
   constexpr int STAGE = kStage<CB>, BLK = STAGE / 16384;  // blocks of 128 k a warp and stage
@@ -271,14 +280,15 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
   uint8_t* xdig = ring + p.stages * STAGE;                            // [pass][blocks][512]
   float* xexp = reinterpret_cast<float*>(xdig + (int64_t)p.pass * p.blocks * (4 * KB));  // [pass][epitch]
   float* part = xexp + p.pass * p.epitch;                             // [PARTS][WARPS][PART]
-  // words that hold the scales of a stage: [AHEAD][warp][block][lane g][row of four]
-  uint32_t(*scales)[WARPS][BLK][32] = reinterpret_cast<uint32_t(*)[WARPS][BLK][32]>(part + PARTS * WARPS * PART);
-  Smem* s = reinterpret_cast<Smem*>(scales + AHEAD);
+  constexpr bool GROUPS = SC != ROW;
+  constexpr int SB = SC == GROUP_BF16 ? 2 : 4;                        // bytes of a scale
+  uint8_t* scales = reinterpret_cast<uint8_t*>(part + PARTS * WARPS * PART);  // [stages][kScales]
+  Smem* s = reinterpret_cast<Smem*>(scales + (GROUPS ? p.stages * kScales<CB> : 0));
   volatile int* abort_flag = &s->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(&s->full[i], 1);
+      mbar_init(&s->full[i], GROUPS ? 33 : 1);
       mbar_init(&s->empty[i], WARPS);
     }
     for (int i = 0; i < PARTS; ++i) {
@@ -364,6 +374,42 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       ++loads;
     }
     if (lane == 0 && loads > 0) wait_drain(&s->xfull, (loads - 1) & 1);
+  } else if (warp == WARPS + 3) {
+    // ---------------- weight scales ----------------
+    // Of a stage's rows in turn, a lane each.  (In the multiplying warps, one
+    // word a row and block, these copies took a sixth of their time and a
+    // quarter of the shared-memory cycles.)
+    if constexpr (GROUPS) {
+      const int per = 2 * slabs, bytes = per * SB, pitch = scale_pitch(bytes);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Item it;
+      for (it.start(p, s); it.left > 0 && ok; it.next(p, s))
+        for (int st = 0; st < steps; ++st) {
+          if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          const int here = min(per, p.blocks - st * per) * SB;  // (behind K: whatever is there)
+          for (int r = lane; r < p.tile; r += 32) {
+            const int64_t first = ((int64_t)it.e * p.N + min(it.n0 + r, p.N - 1)) * p.groups + st * per;
+            const uint8_t* from = static_cast<const uint8_t*>(p.scale) + first * SB;
+            uint8_t* to = scales + stage * kScales<CB> + r * pitch;
+            if (p.scale_copy == 16) {
+              for (int i = 0; i < here; i += 16) cp_async<16>(smem_u32(to + i), from + i);
+            } else if (p.scale_copy == 8) {
+              for (int i = 0; i < here; i += 8) cp_async<8>(smem_u32(to + i), from + i);
+            } else if (p.scale_copy == 4) {
+              for (int i = 0; i < here; i += 4) cp_async<4>(smem_u32(to + i), from + i);
+            } else {
+              for (int i = 0; i < here; i += 2)
+                *reinterpret_cast<uint16_t*>(to + i) = __ldg(reinterpret_cast<const uint16_t*>(from + i));
+            }
+          }
+          if (p.scale_copy > 2) cp_async_arrive(&s->full[stage]);
+          else mbar_arrive(&s->full[stage]);
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+      cp_async_wait_all();  // no copy still writing shared memory at exit
+    }
   } else if (warp == WARPS + 2) {
     // ---------------- outputs ----------------
     if (p.early) pdl_wait();  // before anything is written
@@ -438,35 +484,8 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     // rows behind the last of a pass repeat it (their sums are not stored)
     auto xrow = [&](int c, int odd_half, int rows) { return min(2 * c + odd_half, rows - 1); };
 
-    // Weight scales are copied (cp.async) AHEAD - 1 stages before their use: of
-    // the four rows of lane group g lane t copies row 8 t, and all four lanes
-    // read them back.  A scale read into a register an iteration ahead
-    // stalled each stage for the memory's latency.
-    Item pf;
-    int pf_step = 0, pf_slot = 0;
-    int64_t pf_row = 0;
-    pf.start(p, s);
-    auto fetch = [&]() {
-      if constexpr (GROUPS) {
-        if (pf.left > 0) {
-          if (pf_step == 0) pf_row = ((int64_t)pf.e * p.N + min(pf.n0 + rg * 32 + 8 * t + row, p.N - 1)) * p.groups;
-          const int b = pf_step * 2 * slabs + bi;
-          const uint8_t* from = static_cast<const uint8_t*>(p.scale) + (pf_row + b) * (p.scale_bf16 ? 2 : 4);
-#pragma unroll
-          for (int k = 0; k < BLK; ++k)
-            if (b + k < p.blocks)
-              cp_async_4(&scales[pf_slot][warp][k][lane],
-                         reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(from + k * (p.scale_bf16 ? 2 : 4)) & ~uintptr_t(3)));
-          if (++pf_step == steps) {
-            pf_step = 0;
-            pf.next(p, s);
-          }
-        }
-        cp_async_commit();
-        pf_slot = (pf_slot + 1) & (AHEAD - 1);
-      }
-    };
-    for (int i = 0; i < AHEAD - 1; ++i) fetch();
+    const int pitch = scale_pitch(2 * slabs * SB);
+    const uint8_t* my_scales = scales + (rg * 32 + row) * pitch + bi * SB;  // of row `row`; the others are 8 pitches apart
     if (p.own_digits) {
       constexpr int UN = 4;  // blocks whose values are on their way at a time
       for (int i0 = warp; i0 < p.R * p.blocks; i0 += UN * WARPS) {
@@ -487,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&s->xfull);
     }
-    int stage = 0, now = -1, buf = 0, slot = 0;
+    int stage = 0, now = -1, buf = 0;
     uint32_t phase = 0, loads = 0, pphase = 0;
     bool ok = true;
     Item it;
@@ -508,14 +527,6 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
         xd[c] = xdig + (int64_t)xrow(c, g >> 2, it.rows) * p.blocks * (4 * KB) + (g & 3) * 64 + t * 16;
         xe[c] = xexp + xrow(c, t >> 1, it.rows) * p.epitch;
       }
-      uint32_t upper = 0;  // bit j: the bfloat16 scale of row j and block 0 is a word's upper half
-      if (GROUPS && p.scale_bf16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t first = ((int64_t)it.e * p.N + min(it.n0 + rg * 32 + 8 * j + row, p.N - 1)) * p.groups;
-          upper |= ((uint32_t)(reinterpret_cast<uintptr_t>(p.scale) >> 1) + (uint32_t)first & 1u) << j;
-        }
-      }
       float sum[2][CB][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -524,11 +535,6 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
 #pragma unroll 1
       for (int st = 0; st < steps && ok; ++st) {
         const int b0 = st * 2 * slabs + bi;
-        if constexpr (GROUPS) {
-          fetch();
-          cp_async_wait<AHEAD - 1>();
-          __syncwarp();
-        }
         if (!wait_bounded(&s->full[stage], phase, abort_flag)) { ok = false; break; }
 #pragma unroll
         for (int k = 0; k < BLK; ++k) {
@@ -538,13 +544,13 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
           const int b = min(b0 + k, p.blocks - 1);
           float ws[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};
           if constexpr (GROUPS) {
-            const uint4 u = *reinterpret_cast<const uint4*>(&scales[slot][warp][k][lane & ~3]);
-            const uint32_t word[4] = {u.x, u.y, u.z, u.w};
+            const uint8_t* from = my_scales + stage * kScales<CB> + k * SB;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float f = __uint_as_float(word[j]);
-              if (p.scale_bf16) f = __uint_as_float((upper >> j ^ b) & 1u ? word[j] & 0xFFFF0000u : word[j] << 16);
-              ws[j >> 1][j & 1] = b0 + k < p.blocks ? f : 0.0f;
+              const uint8_t* f = from + 8 * j * pitch;
+              const float v = SC == GROUP_BF16 ? __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(f) << 16)
+                                               : *reinterpret_cast<const float*>(f);
+              ws[j >> 1][j & 1] = b0 + k < p.blocks ? v : 0.0f;
             }
           }
           const uint8_t* d = ring + stage * STAGE + woff[k];
@@ -596,8 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
               }
           }
         }
-        slot = (slot + 1) & (AHEAD - 1);
-        __syncwarp();  // (also: the slot read above may be copied to again)
+        __syncwarp();
         if (lane == 0) mbar_arrive(&s->empty[stage]);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
@@ -616,7 +621,6 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       if (lane == 0) mbar_arrive(&s->pfull[buf]);
       if (++buf == PARTS) { buf = 0; pphase ^= 1; }
     }
-    if constexpr (GROUPS) cp_async_wait<0>();
   }
 }
 
@@ -758,13 +762,13 @@ bool makes_own_digits(bool experts, int64_t R, int64_t N, int64_t K) {
 
 template <int CB>
 constexpr int fixed_bytes() {
-  return 1024 + kParts<CB> * WARPS * 32 * (2 * CB + 1) * 4 + AHEAD * WARPS * (kStage<CB> / 16384) * 128 + (int)sizeof(Smem);
+  return 1024 + kParts<CB> * WARPS * 32 * (2 * CB + 1) * 4 + (int)sizeof(Smem);
 }
 // Bytes of a pass's digits and exponents that every instance has room for, beside 64 KB of weights.
 constexpr int64_t kDigitRoom =
-    SMEM - 65536 - std::max({fixed_bytes<1>(), fixed_bytes<2>(), fixed_bytes<4>()});
+    SMEM - 65536 - 4 * 1536 - std::max({fixed_bytes<1>(), fixed_bytes<2>(), fixed_bytes<4>()});
 
-template <int DT, int CB, bool GROUPS>
+template <int DT, int CB, Scales SC>
 int launch_cfg(MatvecParams p, cudaStream_t stream) {
   const int sms = device_sm_count();
   // rows a pass: what fits beside 64 KB of weights; then as many stages as fit
@@ -774,11 +778,17 @@ int launch_cfg(MatvecParams p, cudaStream_t stream) {
   while (p.tile < 8 * 32 && STAGE / (128 * p.tile) > slabs) p.tile *= 2;
   p.whole = p.K % 256 == 0 && STAGE > 128 * p.tile;  // one slab a stage: the map stays two-dimensional
   const int64_t room = SMEM - fixed_bytes<CB>(), per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
-  const int64_t fit = (room - 65536) / per_row;
+  const int64_t stage = STAGE + (SC != ROW ? kScales<CB> : 0), fit = (room - 65536 / STAGE * stage) / per_row;
   p.pass = (int)(fit < 2 * CB ? fit : 2 * CB);
   if (p.pass > p.R) p.pass = p.R;
-  const int64_t stages = (room - p.pass * per_row) / STAGE;
+  const int64_t stages = (room - p.pass * per_row) / stage;
   p.stages = (int)(stages < MAX_STAGES ? stages : MAX_STAGES);
+  if constexpr (SC != ROW) {  // the widest copies that all rows and stages begin at multiples of
+    constexpr int SB = SC == GROUP_BF16 ? 2 : 4;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.scale) | (uintptr_t)p.groups * SB |
+                          (uintptr_t)(2 * STAGE / (128 * p.tile)) * SB;
+    p.scale_copy = all % 16 == 0 ? 16 : (all % 8 == 0 ? 8 : (all % 4 == 0 ? 4 : 2));
+  }
   const int64_t passes = p.R / p.pass + (p.offsets == nullptr ? 1 : (p.R < p.E ? p.R : p.E));  // at most
   const int64_t items = passes * ((p.N + p.tile - 1) / p.tile);
   if (items > INT32_MAX) return fail(QLIN_ERR_UNSUPPORTED, "matvec_w4: too many outputs");
@@ -786,7 +796,7 @@ int launch_cfg(MatvecParams p, cudaStream_t stream) {
   const int rc = encode_slab_tmap(&tw, p.w, (uint64_t)p.K / 2, (uint64_t)p.E * p.N, 128, p.tile,
                                   p.whole ? STAGE / (128 * p.tile) : 1);
   if (rc) return rc;
-  auto kern = matvec_kernel<DT, CB, GROUPS>;
+  auto kern = matvec_kernel<DT, CB, SC>;
   static std::atomic<uint64_t> attr_devices{0};  // shared-memory limit raised once per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -798,13 +808,14 @@ int launch_cfg(MatvecParams p, cudaStream_t stream) {
     attr_devices.fetch_or(bit);
   }
   e = launch_pdl(kern, dim3((unsigned)(items < sms ? items : sms)), dim3(THREADS),
-                 (size_t)(fixed_bytes<CB>() + p.pass * per_row + p.stages * STAGE), stream, tw, p);
+                 (size_t)(fixed_bytes<CB>() + p.pass * per_row + p.stages * stage), stream, tw, p);
   return e == cudaSuccess ? QLIN_OK : cuda_fail(e, "matvec_w4 launch");
 }
 
 template <int DT, int CB>
 int launch_cb(const MatvecParams& p, cudaStream_t stream) {
-  return p.groups > 1 ? launch_cfg<DT, CB, true>(p, stream) : launch_cfg<DT, CB, false>(p, stream);
+  if (p.groups == 1) return launch_cfg<DT, CB, ROW>(p, stream);
+  return p.scale_bf16 ? launch_cfg<DT, CB, GROUP_BF16>(p, stream) : launch_cfg<DT, CB, GROUP_F32>(p, stream);
 }
 
 template <int DT>
