@@ -419,46 +419,57 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       if (s->begin[0] > 0) zero_bytes(p.out, 0, s->begin[0] * line, thread, count);
       if (s->begin[p.E] < p.R) zero_bytes(p.out, s->begin[p.E] * line, p.R * line, thread, count);
     }
-    int buf = 0, now = -1;
-    uint32_t phase = 0;
-    Item it;
-    for (it.start(p, s); it.left > 0; it.next(p, s)) {
-      if (it.pass != now) {
-        if (now >= 0) {  // done with the exponents of the pass before
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s->xempty);
+    // bias and scale of this lane's column of each 32 of an item, read while the
+    // sums of the one before it are added up
+    constexpr int MAXG = 8;
+    T next_bias[MAXG];
+    float next_scale[MAXG];
+    Item ahead;
+    ahead.start(p, s);
+    auto fetch = [&]() {
+#pragma unroll
+      for (int j = 0; j < MAXG; ++j)
+        if (j < row_groups && ahead.left > 0) {
+          const int64_t at = (int64_t)ahead.e * p.N + min(ahead.n0 + 32 * j + lane, p.N - 1);
+          if (p.bias != nullptr) next_bias[j] = reinterpret_cast<const T*>(p.bias)[at];
+          if constexpr (!GROUPS) next_scale[j] = scale_at(p, at);
         }
-        now = it.pass;
-      }
-      // bias and scale of this lane's column of each 32, read before the sums are waited for
-      constexpr int MAXG = 8;
+    };
+    fetch();
+    int buf = 0, now = -1;
+    uint32_t phase = 0, odd = 0;  // rows of the pass with infinities or NaN
+    while (ahead.left > 0) {
+      const Item it = ahead;
       float bias[MAXG], row_scale[MAXG];
 #pragma unroll
       for (int j = 0; j < MAXG; ++j) {
-        bias[j] = 0.0f;
-        row_scale[j] = 1.0f;
-        if (j < row_groups) {
-          const int64_t at = (int64_t)it.e * p.N + min(it.n0 + 32 * j + lane, p.N - 1);
-          if (p.bias != nullptr) bias[j] = Elem<DT>::to_f(reinterpret_cast<const T*>(p.bias)[at]);
-          if constexpr (!GROUPS) row_scale[j] = scale_at(p, at);
-        }
+        bias[j] = p.bias != nullptr && j < row_groups ? Elem<DT>::to_f(next_bias[j]) : 0.0f;
+        row_scale[j] = next_scale[j];
       }
+      ahead.next(p, s);
+      fetch();
       if (!wait_bounded(&s->pfull[buf], phase, abort_flag)) break;
-      for (int j = 0; j < row_groups; ++j) {
-        const int n = it.n0 + 32 * j + lane;
-        if (n < p.N) {
-          float b = bias[0], rs = row_scale[0];
+      if (it.pass != now) {
+        now = it.pass;
+        odd = s->odd | __ballot_sync(0xffffffffu, lane < it.rows && xexp[min(lane, it.rows - 1) * p.epitch] < 0.0f);
+        if (lane == 0) mbar_arrive(&s->xempty);  // done with the exponents
+      }
 #pragma unroll
-          for (int i = 1; i < MAXG; ++i)
-            if (i == j) { b = bias[i]; rs = row_scale[i]; }
+      for (int j = 0; j < MAXG; ++j) {
+        const int n = it.n0 + 32 * j + lane;
+        if (j < row_groups && n < p.N) {
           const int64_t at = (int64_t)it.e * p.N + n;
-          for (int r = 0; r < it.rows; ++r) {
+#pragma unroll
+          for (int r = 0; r < 2 * CB; ++r) {
+            if (r >= it.rows) break;
             const float* q = part + (buf * WARPS + j) * PART + lane * PITCH + r;
             float v = 0.0f;
-            for (int k = 0; k < share; ++k) v += q[k * row_groups * PART];
-            if (xexp[r * p.epitch] < 0.0f || s->odd >> r & 1u) v += odd_terms<DT>(p, source_row(p, it.r0 + r), at);
-            if constexpr (!GROUPS) v *= rs;
-            if (p.bias != nullptr) v += b;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k)
+              if (k < share) v += q[k * row_groups * PART];
+            if (odd >> r & 1u) v += odd_terms<DT>(p, source_row(p, it.r0 + r), at);
+            if constexpr (!GROUPS) v *= row_scale[j];
+            if (p.bias != nullptr) v += bias[j];
             reinterpret_cast<T*>(p.out)[(int64_t)(it.r0 + r) * p.N + n] = Elem<DT>::from_f(v);
           }
         }
