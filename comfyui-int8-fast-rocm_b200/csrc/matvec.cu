@@ -787,6 +787,11 @@ int launch_cfg(MatvecParams p, cudaStream_t stream) {
   const int slabs = (p.K / 2 + 127) / 128;  // of 128 bytes a row; as few rows a tile as fill whole stages: the most tiles to share out
   p.tile = 32;
   while (p.tile < 8 * 32 && STAGE / (128 * p.tile) > slabs) p.tile *= 2;
+  // With many items 64 rows, whose sums are handed over half as often (N 98304, 4
+  // rows: 45 us, with 32 rows a tile 49; 32 rows of 8 experts, N 8192: 43 and
+  // 45); with few, 32, which share out evenly (N 28672, K 8192: 27 us, 64 rows 30).
+  const int64_t whole_passes = p.R / (2 * CB) > 0 ? p.R / (2 * CB) : 1;
+  if (p.tile == 32 && whole_passes * (p.N / 32) >= 12 * (int64_t)sms) p.tile = 64;
   p.whole = p.K % 256 == 0 && STAGE > 128 * p.tile;  // one slab a stage: the map stays two-dimensional
   const int64_t room = SMEM - fixed_bytes<CB>(), per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
   const int64_t stage = STAGE + (SC != ROW ? kScales<CB> : 0), fit = (room - 65536 / STAGE * stage) / per_row;
@@ -855,11 +860,11 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   // Rows a pass by the rows an expert has on average (how they spread is known
   // on the device only): more columns than rows cost more than a second pass
   // over an expert's weights, which L2 then holds (32 rows of 8 experts, N
-  // 8192, K 4096: 51 us with 4 rows a pass, 59 with 8; 4 rows of one weight, N
-  // 24576: 20 and 28).
-  const int64_t rows = p.offsets == nullptr ? p.R : (p.R < p.E ? 1 : p.R / p.E);
-  if (rows <= 2) return launch_cb<DT, 1>(p, stream);
-  if (rows <= 4) return launch_cb<DT, 2>(p, stream);
+  // 8192, K 4096: 43 us with 4 rows a pass, 47 with 8; 16 rows 32 us with 4 rows
+  // a pass, 34 with 2; 4 rows of one weight, N 24576: 19 and 24).
+  const int64_t sets = p.offsets == nullptr ? 1 : p.E;
+  if (p.offsets == nullptr ? p.R <= 2 : p.R < 2 * sets) return launch_cb<DT, 1>(p, stream);
+  if (p.R < 5 * sets) return launch_cb<DT, 2>(p, stream);
   return launch_cb<DT, 4>(p, stream);
 }
 
