@@ -22,16 +22,20 @@
 //                  128 are exact; digits and scales meet once a block in
 //                  float32.
 //
-// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 16.6 us: about 6 us
-// of launches and latency, then 5 TB/s; N 98304 4.7 TB/s in all.  From 8 rows
-// on the matrix instructions do: 32 columns of digits, 29.5 us at N 24576.
+// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 15.0 us: about 5 us
+// of launches and latency, then 5.4 TB/s (N 98304 5.5 TB/s in all; a copy of the
+// kernel that only loads 5.9).  With more rows the multiplying warps do, two to a
+// scheduler that issue an instruction every four clocks or so (4 rows 18.4 us, 8
+// rows 24.0); 16 of them, with half a stage each, are no faster, since what a
+// warp does once a stage and a tile doubles.
 //
 // matvec_kernel is persistent, a block of threads a SM.  One warp brings the
 // weights by TMA, 32 or 16 KB a stage of 32 rows or more (loads of 64 bytes a
-// row straight into the lanes that need them stayed at 2 TB/s).  One brings an
-// expert's activation digits, which stay in shared memory for all its row
-// tiles.  Eight warps multiply, each 32 rows and one or two blocks of 128 k of
-// a stage.  One adds their sums up, in a fixed order, while they go on.
+// row straight into the lanes that need them stayed at 2 TB/s), one their
+// scales, as many at a time as their alignment allows.  One brings an expert's
+// activation digits, which stay in shared memory for all its row tiles.  Eight
+// warps multiply, each 32 rows and one or two blocks of 128 k of a stage.  One
+// adds their sums up, in a fixed order, while they go on.
 #include <algorithm>
 #include <atomic>
 
@@ -75,6 +79,7 @@ struct MatvecParams {
   int own_digits;         // matvec_kernel makes the digits itself (one pass of one expert)
   int tile;               // weight rows a stage: 32 to 256
   int scale_copy;         // bytes of a copy of weight scales: 16, 8 or 4, 2 for plain loads
+  int x_fours;            // rows of x begin at multiples of four values, and K is one
   int whole;              // a stage is one three-dimensional TMA box (rows are whole slabs of 128 bytes)
   int stages;
   int pass;               // rows of an expert whose digits fit, at most 2 * CB
@@ -103,52 +108,74 @@ __device__ __forceinline__ int64_t source_row(const MatvecParams& p, int r) {
 // Lane l of a warp has k 4l .. 4l + 3 of a block of 128.
 template <int DT>
 __device__ __forceinline__ void load_x4(const MatvecParams& p, int64_t src, int b, int lane, float (&v)[4]) {
+  using T = typename Elem<DT>::T;
+  struct alignas(4 * sizeof(T)) Four { T v[4]; };
   const int k = b * KB + 4 * lane;
-  const typename Elem<DT>::T* x = reinterpret_cast<const typename Elem<DT>::T*>(p.x) + src * p.ldx + k;
+  const T* x = reinterpret_cast<const T*>(p.x) + src * p.ldx + k;
+  if (p.x_fours) {
+    Four f;
+    if (src >= 0 && k < p.K) f = *reinterpret_cast<const Four*>(x);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = src >= 0 && k + i < p.K ? Elem<DT>::to_f(x[i]) : 0.0f;
+    for (int i = 0; i < 4; ++i) v[i] = src >= 0 && k < p.K ? Elem<DT>::to_f(f.v[i]) : 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = src >= 0 && k + i < p.K ? Elem<DT>::to_f(x[i]) : 0.0f;
+  }
 }
-// The block's digits to out [half][digit][lane t][16 bytes], 2^e to *exp;
-// whether there are infinities or NaN (which add nothing here, see odd_terms).
-// The matrix instruction meets a word of eight nibbles as its even and its
-// odd ones, so the digits of k 0 2 4 6 and of 1 3 5 7 of each eight lie
-// together; lane t of the product reads words 4t .. 4t + 3 of a block, two at
-// a time.
-__device__ __forceinline__ bool make_digits(float (&v)[4], int lane, void* out, float* exp) {
-  uint32_t big = 0;
-  bool odd = false;
+// The digits of UN blocks to out[u] [half][digit][lane t][16 bytes], 2^e to
+// *exp[u]; which of the blocks (bit u) have infinities or NaN (which add
+// nothing here, see odd_terms).  The matrix instruction meets a word of eight
+// nibbles as its even and its odd ones, so the digits of k 0 2 4 6 and of
+// 1 3 5 7 of each eight lie together; lane t of the product reads words 4t ..
+// 4t + 3 of a block, two at a time.
+template <int UN>
+__device__ __forceinline__ uint32_t make_digits(float (&v)[UN][4], int lane, void* const (&out)[UN],
+                                                float* const (&exp)[UN]) {
+  uint32_t big[UN], odd = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (!(fabsf(v[i]) <= 3.402823466e38f)) {
-      odd = true;
-      v[i] = 0.0f;
-    }
-    big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  }
-  big = __reduce_max_sync(0xffffffffu, big);
-  const int e = max((int)(big >> 23), 1) - 127;  // |x| < 2^(e + 1)
-  // 2^(29 - e) in two factors, each a float
-  const float f1 = pow2((29 - e) >> 1), f2 = pow2(29 - e - ((29 - e) >> 1));
-  uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit q of the four k
+  for (int u = 0; u < UN; ++u) {
+    big[u] = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    int X = __float2int_rn(__fmul_rn(__fmul_rn(v[i], f1), f2));
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      d[q] |= ((uint32_t)X & 0xFFu) << (8 * i);
-      X = (X + 128) >> 8;  // the signed digit taken off
+    for (int i = 0; i < 4; ++i) {
+      uint32_t m = __float_as_uint(v[u][i]) & 0x7FFFFFFFu;
+      if (m >= 0x7F800000u) {
+        odd |= 1u << u;
+        v[u][i] = 0.0f;
+        m = 0;
+      }
+      big[u] = max(big[u], m);
     }
   }
+#pragma unroll
+  for (int u = 0; u < UN; ++u) big[u] = __reduce_max_sync(0xffffffffu, big[u]);
   const int word = lane >> 1;  // of eight k: the even lane stores its even ones, the odd lane its odd ones
-  uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + (word >> 1 & 1) * 256 + (word >> 2) * 16 +
-                                             (word & 1) * 8 + (lane & 1) * 4);
+  const int at = (word >> 1 & 1) * 256 + (word >> 2) * 16 + (word & 1) * 8 + (lane & 1) * 4;
+  const uint32_t mine = lane & 1 ? 0x7531u : 0x6420u, theirs = lane & 1 ? 0x6420u : 0x7531u;
+  const uint32_t low = lane & 1 ? 0x1054u : 0x5410u, high = lane & 1 ? 0x3276u : 0x7632u;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, d[q], 1);
-    to[q * 16] = lane & 1 ? __byte_perm(other, d[q], 0x7531) : __byte_perm(d[q], other, 0x6420);
+  for (int u = 0; u < UN; ++u) {
+    const int e = max((int)(big[u] >> 23), 1) - 127;  // |x| < 2^(e + 1)
+    // 2^(29 - e) in two factors, each a float
+    const float f1 = pow2((29 - e) >> 1), f2 = pow2(29 - e - ((29 - e) >> 1));
+    uint32_t d[4];  // a k's signed digits: X + 128 (1 + 256 + 65536) has them 128 up as its bytes
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      d[i] = (uint32_t)(__float2int_rn(__fmul_rn(__fmul_rn(v[u][i], f1), f2)) + 0x00808080) ^ 0x00808080u;
+    const uint32_t a = __byte_perm(d[0], d[1], 0x5140), b = __byte_perm(d[2], d[3], 0x5140);
+    const uint32_t c = __byte_perm(d[0], d[1], 0x7362), f = __byte_perm(d[2], d[3], 0x7362);
+    const uint32_t q[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, f, 0x5410),
+                           __byte_perm(c, f, 0x7632)};  // digit q of the four k
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out[u]) + at);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {  // two digits an exchange
+      const uint32_t keep = __byte_perm(q[i], q[i + 1], mine);
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, __byte_perm(q[i], q[i + 1], theirs), 1);
+      to[i * 16] = __byte_perm(keep, other, low);
+      to[(i + 1) * 16] = __byte_perm(keep, other, high);
+    }
+    if (lane == 0) *exp[u] = pow2(e);
   }
-  if (lane == 0) *exp = pow2(e);
-  return __any_sync(0xffffffffu, odd);
+  return __reduce_or_sync(0xffffffffu, odd);
 }
 
 // One block a row, a warp 128 k at a time.
@@ -160,9 +187,9 @@ __global__ void __launch_bounds__(1024) split_kernel(MatvecParams p) {
   const int64_t r = blockIdx.x;
   bool odd = false;
   for (int b = warp; b < p.blocks; b += blockDim.x >> 5) {
-    float v[4];
-    load_x4<DT>(p, r, b, lane, v);
-    odd |= make_digits(v, lane, p.digits + (r * p.blocks + b) * (4 * KB), p.exps + r * p.epitch + b);
+    float v[1][4];
+    load_x4<DT>(p, r, b, lane, v[0]);
+    odd |= make_digits<1>(v, lane, {p.digits + (r * p.blocks + b) * (4 * KB)}, {p.exps + r * p.epitch + b}) != 0;
   }
   if (__syncthreads_or(odd))
     for (int b = threadIdx.x; b < p.blocks; b += blockDim.x) p.exps[r * p.epitch + b] *= -1.0f;
@@ -303,6 +330,23 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
   }
   pdl_launch_dependents();
   if (!p.early) pdl_wait();
+  struct alignas(4 * sizeof(T)) Four { T v[4]; };  // a lane's values of a block
+  if (p.own_digits && warp < WARPS) {
+    // The values, where their digits will be, asked for before the first
+    // weights: behind those a load waits until the ring is full (2 us).
+#pragma unroll 1
+    for (int i = warp; i < p.R * p.blocks; i += WARPS) {
+      const int r = i / p.blocks, k = (i - r * p.blocks) * KB + 4 * lane;
+      const int64_t src = source_row(p, r);
+      const T* from = reinterpret_cast<const T*>(p.x) + src * p.ldx + k;
+      Four* to = reinterpret_cast<Four*>(xdig + (int64_t)i * (4 * KB)) + lane;
+      if (p.x_fours && src >= 0 && k < p.K) {
+        cp_async<4 * sizeof(T)>(smem_u32(to), from);
+      } else {
+        for (int j = 0; j < 4; ++j) to->v[j] = src >= 0 && k + j < p.K ? from[j] : Elem<DT>::from_f(0.0f);
+      }
+    }
+  }
   if (p.offsets != nullptr) {
     for (int e = threadIdx.x; e <= p.E; e += THREADS) s->begin[e] = min(max(p.offsets[e], 0), p.R);
   } else if (threadIdx.x < 2) {
@@ -498,21 +542,19 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     const int pitch = scale_pitch(2 * slabs * SB);
     const uint8_t* my_scales = scales + (rg * 32 + row) * pitch + bi * SB;  // of row `row`; the others are 8 pitches apart
     if (p.own_digits) {
-      constexpr int UN = 4;  // blocks whose values are on their way at a time
-      for (int i0 = warp; i0 < p.R * p.blocks; i0 += UN * WARPS) {
-        float v[UN][4];
+      cp_async_wait_all();
+      __syncwarp();
+#pragma unroll 1  // (code that runs once waits for its instructions)
+      for (int i = warp; i < p.R * p.blocks; i += WARPS) {
+        const int r = i / p.blocks;
+        uint8_t* block = xdig + (int64_t)i * (4 * KB);
+        const Four f = reinterpret_cast<const Four*>(block)[lane];
+        float v[1][4];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int i = i0 + u * WARPS, r = i / p.blocks;
-          load_x4<DT>(p, i < p.R * p.blocks ? source_row(p, r) : -1, i - r * p.blocks, lane, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int i = i0 + u * WARPS, r = i / p.blocks;
-          if (i < p.R * p.blocks &&
-              make_digits(v[u], lane, xdig + (int64_t)i * (4 * KB), xexp + r * p.epitch + i - r * p.blocks) && lane == 0)
-            atomicOr(&s->odd, 1u << r);
-        }
+        for (int j = 0; j < 4; ++j) v[0][j] = Elem<DT>::to_f(f.v[j]);
+        __syncwarp();  // read by all before the digits take their place
+        if (make_digits<1>(v, lane, {block}, {xexp + r * p.epitch + i - r * p.blocks}) && lane == 0)
+          atomicOr(&s->odd, 1u << r);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s->xfull);
@@ -762,14 +804,11 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
   }
 }
 
-// Few values and few weights: every block makes the digits itself.  That takes
-// the device up to a microsecond longer (one row, N 4096, K 4096: 8.2 us, with
-// split_kernel 7.4) but saves a launch and a workspace, 6 of 18 us of a call;
-// with more weights the launch pays, since the ring fills meanwhile (N 24576:
-// 16.6 us, with own digits 19.1).
-bool makes_own_digits(bool experts, int64_t R, int64_t N, int64_t K) {
-  return !experts && R <= 8 && R * K <= 8192 && N * K <= (int64_t)32 << 20;
-}
+// Few values: every block of threads makes the digits itself, which saves a
+// launch and a workspace, 4 of 19 us of a call.  On the device one row of K 4096
+// takes as long as with split_kernel (N 24576: 15.0 us, 14.7), two rows 0.3 to
+// 1.2 us longer, 4 rows 3 to 4 us: more than the call saves in a graph.
+bool makes_own_digits(bool experts, int64_t R, int64_t K) { return !experts && R <= 8 && R * K <= 8192; }
 
 template <int CB>
 constexpr int fixed_bytes() {
@@ -839,7 +878,7 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   cudaError_t e;
   const int64_t per_row = (int64_t)p.blocks * (4 * KB) + p.epitch * 4;
   const bool fast = aligned && per_row <= kDigitRoom;  // (the latter: K up to about 32,000)
-  p.own_digits = fast && makes_own_digits(p.offsets != nullptr, p.R, p.N, p.K);
+  p.own_digits = fast && makes_own_digits(p.offsets != nullptr, p.R, p.K);
   p.early = !p.own_digits && p.Rx > 0;
   if (p.early) {
     const int threads = 32 * (p.blocks < 32 ? p.blocks : 32);
@@ -886,7 +925,7 @@ Workspace workspace_layout(int64_t Rx, int64_t K) {
 }  // namespace
 
 size_t matvec_workspace_bytes(const uint8_t* w, bool experts, int64_t R, int64_t Rx, int64_t N, int64_t K) {
-  if (aligned_weights(w, K) && makes_own_digits(experts, R, N, K)) return 0;
+  if (aligned_weights(w, K) && makes_own_digits(experts, R, K)) return 0;
   return workspace_layout(Rx, K).bytes;
 }
 
@@ -915,6 +954,8 @@ int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8
   p.digits = static_cast<int8_t*>(workspace);
   p.exps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + l.exps);
   p.epitch = (int)l.epitch;
+  const int64_t four = 4 * (dt == DT_F32 ? 4 : 2);
+  p.x_fours = K % 4 == 0 && ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % four == 0;
   const bool aligned = aligned_weights(w, K);
   if (dt == DT_BF16) return launch_dt<DT_BF16>(p, aligned, stream);
   if (dt == DT_F16) return launch_dt<DT_F16>(p, aligned, stream);

@@ -409,6 +409,48 @@ def test_matvec_depth_at_the_limit_of_shared_memory(pkg, K, M):
 
 
 @on_gpu
+@pytest.mark.parametrize("M,groups", [(1, True), (3, False), (6, True)])
+def test_matvec_many_columns(pkg, M, groups):
+    """Tiles of 64 rows, the last one partly filled; every 97th column and the last ones are looked at."""
+    Nn, K = 56_900, 2048
+    x, p, s, b = matvec_inputs(26, M, None, Nn, K, groups, "bf16", True)
+    got = run_matvec(pkg, x, p, s, b).cpu()
+    at = torch.cat((torch.arange(0, Nn - 80, 97), torch.arange(Nn - 80, Nn)))
+    assert_matvec(got[:, at], *matvec_ref(x, p[at], s[at], b[at], None, None), K)
+
+
+@on_gpu
+@pytest.mark.parametrize("sdt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [256, 384, 512, 1024, 2048, 4224])
+@pytest.mark.parametrize("off", [0, 1, 2, 4])
+def test_matvec_scales_of_any_alignment(pkg, sdt, K, off):
+    """The scales come 16, 8, 4 or 2 bytes at a time."""
+    x, p, s, b = matvec_inputs(27 + K, 5, 2, 70, K, True, "f16", True, sdt)
+    room = torch.full((s.numel() + 8,), math.nan, dtype=sdt, device="cuda")
+    view = room[off:off + s.numel()].view(s.shape)
+    view.copy_(s)
+    offsets = torch.tensor([0, 1, 5], dtype=torch.int32, device="cuda")
+    got = pkg.ops.matvec_w4(x.cuda(), p.cuda(), view, b.cuda(), offsets)
+    assert_matvec(got, *matvec_ref(x, p, s, b, [0, 1, 5], None), K)
+
+
+@on_gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("off,pad", [(0, 0), (1, 0), (4, 4), (4, 1)])
+def test_matvec_few_values_of_any_alignment(pkg, dt, off, pad):
+    """Rows of x that begin at multiples of four values and others, in the call that makes its digits itself."""
+    K = 1056
+    x, p, s, b = matvec_inputs(28, 3, None, 90, K, False, dt, True)
+    room = torch.full((off + 3 * (K + pad) + 4,), math.nan, dtype=x.dtype, device="cuda")
+    view = room[off:off + 3 * (K + pad)].view(3, K + pad)[:, :K]
+    view.copy_(x)
+    assert_matvec(pkg.ops.matvec_w4(view, p.cuda(), s.cuda(), b.cuda()), *matvec_ref(x, p, s, b, None, None), K)
+    rows = torch.tensor([2, -1, 0, 7, 2], dtype=torch.int32)
+    got = pkg.ops.matvec_w4(view, p.cuda(), s.cuda(), b.cuda(), None, rows.cuda())
+    assert_matvec(got, *matvec_ref(x, p, s, b, None, rows), K)
+
+
+@on_gpu
 @pytest.mark.parametrize("K", [256, 258])  # both kernels (258: one scale a row)
 @pytest.mark.parametrize("xe,se", [(100, -120), (-110, 100), (0, -126), (127, -126)])
 def test_matvec_scales_far_from_one(pkg, K, xe, se):
