@@ -118,8 +118,8 @@ def convrot_w4a16_forward(x: Tensor, qweight: Tensor, wscales: Tensor, bias, con
     """:func:`convrot_w4a4_forward` for few rows (a modulation or embedding
     linear, whose rows are the batch's samples) with the activation kept in
     ``compute_dtype`` instead of quantised to int4; ``wscales`` [N], or
-    [N, K/128] for group-128 weights.  Up to about 8 rows also the faster of
-    the two (one row, K 4096, N 24576, without the rotation: 15 us against 32);
+    [N, K/128] for group-128 weights.  Up to 8 rows also the faster of
+    the two (one row, K 4096, N 24576, without the rotation: 14 us against 32);
     no counterpart in the reference."""
     if x.shape[-1] != qweight.shape[-1] * 2:
         raise ValueError(f"Input K={x.shape[-1]} does not match packed qweight K={qweight.shape[-1] * 2}")
