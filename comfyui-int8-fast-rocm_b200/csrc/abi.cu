@@ -187,6 +187,29 @@ QLIN_API int qlin_selftest_gemm_stall(const int8_t* a, const float* a_scale, con
   return launch_gemm_stall(a, a_scale, w, w_scale, out, M, N, K, stall_kb, static_cast<cudaStream_t>(stream));
 }
 
+QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, const float* w_scale, int group,
+                                        void* out, int64_t R, int64_t N, int64_t K, void* workspace,
+                                        uint64_t workspace_bytes, int which, int64_t stage, void* stream) {
+  QLIN_RANGE();
+  if (R <= 0 || N <= 0 || K <= 0 || K > 16384 || R > INT32_MAX - 256 || N > INT32_MAX - 256)
+    return fail(QLIN_ERR_INVALID_ARG, "bad shape");
+  if (which != 0) return fail(QLIN_ERR_INVALID_ARG, "which must be 0 (weights)");
+  if (stage < 0 || stage > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "stage out of range");
+  if (group != 0 && group != 128) return fail(QLIN_ERR_UNSUPPORTED, "int4 group must be 0 (per row) or 128");
+  if (K % (group ? 128 : 32)) return fail(QLIN_ERR_INVALID_ARG, "K must be a multiple of 32, of 128 with groups");
+  if (!x || !w_packed || !w_scale || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
+  const uint64_t need = matvec_workspace_bytes(reinterpret_cast<const uint8_t*>(w_packed), false, R, R, N, K);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(QLIN_ERR_INVALID_ARG, "workspace of " + std::to_string(need) + " bytes needed");
+  if (!aligned16(w_packed) || !aligned16(workspace) || !aligned16(out))
+    return fail(QLIN_ERR_ALIGNMENT, "operands must be 16-byte aligned");
+  int rc = check_device();
+  if (rc) return rc;
+  return launch_matvec_w4(DT_BF16, x, R, K, reinterpret_cast<const uint8_t*>(w_packed), w_scale, DT_F32,
+                          group ? (int)(K / group) : 1, nullptr, 1, nullptr, nullptr, out, R, N, K, workspace,
+                          static_cast<cudaStream_t>(stream), (int)stage);
+}
+
 QLIN_API int qlin_quant_act_int8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int rot_kind,
                                  int rot_group, float rot_c, int8_t* q, float* scale, void* stream) {
   QLIN_RANGE();

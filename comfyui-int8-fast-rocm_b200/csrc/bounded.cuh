@@ -33,6 +33,12 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, vol
   }
 }
 
+// The same by all lanes of a warp, which go by one verdict: a wait that runs
+// out must not part lanes that meet at shuffles and votes later on.
+__device__ __forceinline__ bool wait_bounded_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort));
+}
+
 // Waits (whatever the abort flag says) for asynchronous work issued earlier.
 __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
   const uint64_t limit = *reinterpret_cast<volatile uint64_t*>(&g_tu_wait_limit_ns);

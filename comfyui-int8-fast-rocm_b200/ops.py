@@ -932,3 +932,20 @@ def selftest_gemm_stall(a_q, a_scale, w_q, w_scale, stall_kb: int = 0) -> torch.
     N.call("qlin_selftest_gemm_stall", _ptr(a_q), _ptr(a_scale.float().contiguous()), _ptr(w_q),
            _ptr(w_scale.float().contiguous()), _ptr(out), M, Nn, K, int(stall_kb), _stream(a_q))
     return out
+
+
+def selftest_matvec_stall(x, w_packed, w_scale, which: int = 0, stage: int = 0) -> torch.Tensor:
+    """:func:`matvec_w4` of contiguous bf16 ``x`` without experts whose
+    producer (``which`` 0: of the weights) never fills stage ``stage`` of each
+    block of threads: the wait for it runs out and the kernel returns with
+    error bit 0 set.  Returns the (partly written) output."""
+    R, K = x.shape
+    Nn = w_packed.shape[0]
+    out = torch.empty((R, Nn), dtype=torch.bfloat16, device=x.device)
+    st = _stream(x)
+    need = ctypes.c_uint64(0)
+    N.call("qlin_matvec_w4_workspace", w_packed.data_ptr(), 0, R, R, Nn, K, ctypes.addressof(need))
+    ws = x.new_empty((need.value,), dtype=torch.uint8) if need.value else None
+    N.call("qlin_selftest_matvec_stall", x.data_ptr(), w_packed.data_ptr(), w_scale.data_ptr(),
+           128 if w_scale.dim() == 2 else 0, out.data_ptr(), R, Nn, K, _ptr(ws), need.value, int(which), int(stage), st)
+    return out

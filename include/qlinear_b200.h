@@ -113,6 +113,17 @@ QLIN_API int qlin_selftest_wait_timeout(int which, void* stream);
 QLIN_API int qlin_selftest_gemm_stall(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale,
                                       void* out, int64_t M, int64_t N, int64_t K, int64_t stall_kb, void* stream);
 
+/* Self-test of the 4-bit matrix-vector product's abort path: qlin_matvec_w4
+ * of bf16 x [R, K] without experts, gathered rows or a bias, K <= 16384 and a
+ * multiple of 32, 16-byte aligned weights.  which 0: the TMA producer of each
+ * block of threads leaves its stage `stage` (counted from 0) unfilled, so that
+ * the multiplying warps' wait for it runs out after the limit: error bit 0 is
+ * set and the kernel returns with `out` partly written.  A stage that no block
+ * reaches changes nothing. */
+QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, const float* w_scale, int group,
+                                        void* out, int64_t R, int64_t N, int64_t K, void* workspace,
+                                        uint64_t workspace_bytes, int which, int64_t stage, void* stream);
+
 /* ---- (a) activation quantisation, fused with the ConvRot rotation -------- */
 
 /* Per-token int8 quantisation of x[M,K] (dtype x_dtype in {BF16,F16,F32}),

@@ -944,3 +944,15 @@ def test_abi_refusals(pkg):
     assert lib.qlin_matvec_w4_workspace(16, 0, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value == 0
     assert lib.qlin_matvec_w4_workspace(17, 0, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value > 0
     assert lib.qlin_matvec_w4_workspace(16, 1, 1, 1, 8, 256, ctypes.addressof(n)) == 0 and n.value > 0
+
+
+def test_matvec_stall_refusals(pkg):
+    N = pkg._native
+    lib = N.load()
+    bad, align, unsup = N.ERR_INVALID_ARG, N.ERR_ALIGNMENT, N.ERR_UNSUPPORTED
+    st = lambda x=16, w=16, R=40, Nn=8, K=256, group=128, ws=16, nws=2 ** 20, which=0, stage=0: \
+        lib.qlin_selftest_matvec_stall(x, w, 16, group, 16, R, Nn, K, ws, nws, which, stage, None)
+    assert st(x=None) == st(R=0) == st(Nn=0) == st(K=0) == st(K=16512) == st(K=160) == st(K=48, group=0) == bad
+    assert st(which=-1) == st(stage=-1) == st(ws=None) == st(nws=40 * 256) == bad
+    assert st(group=64) == unsup
+    assert st(w=24) == st(ws=24) == align

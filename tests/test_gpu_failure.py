@@ -71,3 +71,30 @@ def test_set_wait_limit_rejects_out_of_range(pkg):
         pkg.ops.set_wait_limit(10)  # below 1 us
     with pytest.raises(NativeError):
         pkg.ops.set_wait_limit(120 * 10**9)
+
+
+def _matvec(P, R, N, K, grouped, seed=43):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, K, generator=g).to(torch.bfloat16).cuda()
+    p = torch.randint(-128, 128, (N, K // 2), generator=g).to(torch.int8).cuda()
+    s = (torch.rand(N, K // 128, generator=g) if grouped else torch.rand(N, generator=g)).cuda()
+    return x, p, s
+
+
+# rows of one, two and four column blocks, digits made in the kernel (R * K <= 8192) and before it
+@pytest.mark.parametrize("R,K,stage", [(1, 1024, 0), (1, 8192, 2), (2, 16384, 3), (4, 4096, 1), (8, 2048, 0), (20, 4096, 5)])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_matvec_stall_aborts_and_recovers(short_limit, R, K, stage, grouped):
+    P, N = short_limit, 9000
+    x, p, s = _matvec(P, R, N, K, grouped)
+    want = P.ops.matvec_w4(x, p, s)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
+    P.ops.selftest_matvec_stall(x, p, s, 0, stage)
+    torch.cuda.synchronize()
+    bits = P.ops.device_error()
+    assert bits & 1, bits
+    assert not bits & 4, bits  # the loads in flight were waited for
+    assert torch.equal(P.ops.matvec_w4(x, p, s), want)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
