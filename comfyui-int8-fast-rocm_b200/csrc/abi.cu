@@ -193,7 +193,8 @@ QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, c
   QLIN_RANGE();
   if (R <= 0 || N <= 0 || K <= 0 || K > 16384 || R > INT32_MAX - 256 || N > INT32_MAX - 256)
     return fail(QLIN_ERR_INVALID_ARG, "bad shape");
-  if (which != 0) return fail(QLIN_ERR_INVALID_ARG, "which must be 0 (weights)");
+  if (which != 0 && (which != 1 || group != 128))
+    return fail(QLIN_ERR_INVALID_ARG, "which must be 0 (weights) or, with groups, 1 (scales)");
   if (stage < 0 || stage > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "stage out of range");
   if (group != 0 && group != 128) return fail(QLIN_ERR_UNSUPPORTED, "int4 group must be 0 (per row) or 128");
   if (K % (group ? 128 : 32)) return fail(QLIN_ERR_INVALID_ARG, "K must be a multiple of 32, of 128 with groups");
@@ -207,7 +208,7 @@ QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, c
   if (rc) return rc;
   return launch_matvec_w4(DT_BF16, x, R, K, reinterpret_cast<const uint8_t*>(w_packed), w_scale, DT_F32,
                           group ? (int)(K / group) : 1, nullptr, 1, nullptr, nullptr, out, R, N, K, workspace,
-                          static_cast<cudaStream_t>(stream), (int)stage);
+                          static_cast<cudaStream_t>(stream), which == 0 ? (int)stage : -1, which == 1 ? (int)stage : -1);
 }
 
 QLIN_API int qlin_quant_act_int8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int rot_kind,

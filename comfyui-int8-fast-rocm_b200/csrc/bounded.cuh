@@ -39,9 +39,11 @@ __device__ __forceinline__ bool wait_bounded_warp(uint64_t* bar, uint32_t parity
   return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort));
 }
 
-// Waits (whatever the abort flag says) for asynchronous work issued earlier.
+// Waits (whatever the abort flag says) for asynchronous work issued earlier,
+// twice the limit at most: a role that owes the barrier arrivals may first
+// have to run out its own wait.
 __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
-  const uint64_t limit = *reinterpret_cast<volatile uint64_t*>(&g_tu_wait_limit_ns);
+  const uint64_t limit = 2 * *reinterpret_cast<volatile uint64_t*>(&g_tu_wait_limit_ns);
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
     if (globaltimer_ns() - t0 > limit) {
@@ -49,6 +51,21 @@ __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
       return;
     }
   }
+}
+
+// A count that another role sets (from -1) when it leaves its loop, which it
+// does within the limit of its own last wait; -1 if it has not by twice that.
+__device__ __forceinline__ int wait_value(const volatile int* value) {
+  const uint64_t limit = 2 * *reinterpret_cast<volatile uint64_t*>(&g_tu_wait_limit_ns);
+  const uint64_t t0 = globaltimer_ns();
+  int v;
+  while ((v = *value) < 0) {
+    if (globaltimer_ns() - t0 > limit) {
+      atomicOr(&g_tu_error_bits, 4u);
+      break;
+    }
+  }
+  return v;
 }
 
 int set_tu_wait_limit(uint64_t ns) {

@@ -181,7 +181,8 @@ int set_grouped_wait_limit(uint64_t ns);
 int read_grouped_error(cudaStream_t stream, uint32_t* bits);
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
-                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall_weights = -1);
+                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall_weights = -1,
+                     int stall_scales = -1);
 size_t matvec_workspace_bytes(const uint8_t* w, bool experts, int64_t R, int64_t Rx, int64_t N, int64_t K);
 int set_matvec_wait_limit(uint64_t ns);
 int read_matvec_error(cudaStream_t stream, uint32_t* bits);

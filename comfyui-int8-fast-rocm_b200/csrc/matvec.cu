@@ -84,6 +84,7 @@ struct MatvecParams {
   int stages;
   int pass;               // rows of an expert whose digits fit, at most 2 * CB
   int stall_weights;      // self-test: the stage, counted from 0, that a block's producer leaves out; else -1
+  int stall_scales;       // and the one at which the scales' warp waits in vain
   // of split_kernel, in the caller's workspace
   int8_t* digits;         // [Rx, blocks, half, digit, lane t, 16]
   float* exps;            // [Rx, epitch] 2^e, negative where the row has infinities or NaN
@@ -223,8 +224,9 @@ __device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, 
 }
 
 struct Smem {  // behind the ring, the digits, the partial sums and the scales
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], pfull[3], pempty[3], xfull, xempty;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], pfull[3], pempty[3], xfull, xempty, never;
   int abort_flag;
+  int fills;                   // stages the producer filled, once it has left its loop; -1 before
   uint32_t odd;                // own_digits: rows with infinities or NaN
   int first_items, first_pass, first_n0;  // this block of threads' items: how many, and where they begin
   int begin[MAX_EXPERTS + 1];  // first row of each expert, ascending within [0, R]
@@ -313,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
   uint8_t* scales = reinterpret_cast<uint8_t*>(part + PARTS * WARPS * PART);  // [stages][kScales]
   Smem* s = reinterpret_cast<Smem*>(scales + (GROUPS ? p.stages * kScales<CB> : 0));
   volatile int* abort_flag = &s->abort_flag;
+  volatile int* fills_at_end = &s->fills;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
@@ -325,7 +328,9 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     }
     mbar_init(&s->xfull, p.own_digits ? WARPS : 1);
     mbar_init(&s->xempty, WARPS + 1);
+    mbar_init(&s->never, 1);
     *abort_flag = 0;
+    *fills_at_end = -1;
     s->odd = 0u;
     fence_mbar_init();
   }
@@ -392,6 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
           if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
       }
+      *fills_at_end = fills;
       armed.drain(s->full);  // no load still writing shared memory at exit
     }
   } else if (warp == WARPS + 1) {
@@ -428,13 +434,17 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     // quarter of the shared-memory cycles.)
     if constexpr (GROUPS) {
       const int per = 2 * slabs, bytes = per * SB, pitch = scale_pitch(bytes);
-      int stage = 0;
+      int stage = 0, fills = 0;
       uint32_t phase = 0;
       bool ok = true;
       Item it;
       for (it.start(p, s); it.left > 0 && ok; it.next(p, s))
         for (int st = 0; st < steps; ++st) {
-          if (!wait_bounded_warp(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          if (!wait_bounded_warp(fills != p.stall_scales ? &s->empty[stage] : &s->never,
+                                 fills != p.stall_scales ? phase ^ 1 : 0, abort_flag)) {
+            ok = false;
+            break;
+          }
           const int here = min(per, p.blocks - st * per) * SB;  // (behind K: whatever is there)
           for (int r = lane; r < p.tile; r += 32) {
             const int64_t first = ((int64_t)it.e * p.N + min(it.n0 + r, p.N - 1)) * p.groups + st * per;
@@ -453,8 +463,17 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
           }
           if (p.scale_copy > 2) cp_async_arrive(&s->full[stage]);
           else mbar_arrive(&s->full[stage]);
+          ++fills;
           if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
+      if (!ok) {
+        // The producer waits for its loads at the barriers that this warp
+        // arrives at too: it gets the arrivals of the stages filled since.
+        for (const int n = wait_value(fills_at_end); fills < n; ++fills) {
+          mbar_arrive(&s->full[stage]);
+          if (++stage == p.stages) stage = 0;
+        }
+      }
       cp_async_wait_all();  // no copy still writing shared memory at exit
     }
   } else if (warp == WARPS + 2) {
@@ -939,7 +958,8 @@ size_t matvec_workspace_bytes(const uint8_t* w, bool experts, int64_t R, int64_t
 
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
                      int groups, const int32_t* offsets, int64_t E, const int32_t* x_rows, const void* bias, void* out,
-                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall_weights) {
+                     int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall_weights,
+                     int stall_scales) {
   if (device_sm_count() < 1) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
   const Workspace l = workspace_layout(Rx, K);
   MatvecParams p{};
@@ -963,6 +983,7 @@ int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8
   p.exps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + l.exps);
   p.epitch = (int)l.epitch;
   p.stall_weights = stall_weights;
+  p.stall_scales = stall_scales;
   const int64_t four = 4 * (dt == DT_F32 ? 4 : 2);
   p.x_fours = K % 4 == 0 && ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % four == 0;
   const bool aligned = aligned_weights(w, K);

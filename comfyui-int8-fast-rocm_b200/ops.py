@@ -936,9 +936,9 @@ def selftest_gemm_stall(a_q, a_scale, w_q, w_scale, stall_kb: int = 0) -> torch.
 
 def selftest_matvec_stall(x, w_packed, w_scale, which: int = 0, stage: int = 0) -> torch.Tensor:
     """:func:`matvec_w4` of contiguous bf16 ``x`` without experts whose
-    producer (``which`` 0: of the weights) never fills stage ``stage`` of each
-    block of threads: the wait for it runs out and the kernel returns with
-    error bit 0 set.  Returns the (partly written) output."""
+    producer (``which`` 0: of the weights; 1: of group scales) never fills
+    stage ``stage`` of each block of threads: the wait for it runs out and the
+    kernel returns with error bit 0 set.  Returns the (partly written) output."""
     R, K = x.shape
     Nn = w_packed.shape[0]
     out = torch.empty((R, Nn), dtype=torch.bfloat16, device=x.device)

@@ -118,8 +118,8 @@ QLIN_API int qlin_selftest_gemm_stall(const int8_t* a, const float* a_scale, con
  * multiple of 32, 16-byte aligned weights.  which 0: the TMA producer of each
  * block of threads leaves its stage `stage` (counted from 0) unfilled, so that
  * the multiplying warps' wait for it runs out after the limit: error bit 0 is
- * set and the kernel returns with `out` partly written.  A stage that no block
- * reaches changes nothing. */
+ * set and the kernel returns with `out` partly written.  which 1 (group 128):
+ * the warp that brings the weight scales waits in vain before that stage.  A stage that no block reaches changes nothing. */
 QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, const float* w_scale, int group,
                                         void* out, int64_t R, int64_t N, int64_t K, void* workspace,
                                         uint64_t workspace_bytes, int which, int64_t stage, void* stream);

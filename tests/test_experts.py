@@ -956,3 +956,4 @@ def test_matvec_stall_refusals(pkg):
     assert st(which=-1) == st(stage=-1) == st(ws=None) == st(nws=40 * 256) == bad
     assert st(group=64) == unsup
     assert st(w=24) == st(ws=24) == align
+    assert st(which=1, group=0) == st(which=2) == bad

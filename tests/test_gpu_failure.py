@@ -98,3 +98,20 @@ def test_matvec_stall_aborts_and_recovers(short_limit, R, K, stage, grouped):
     assert torch.equal(P.ops.matvec_w4(x, p, s), want)
     torch.cuda.synchronize()
     assert P.ops.device_error() == 0
+
+
+@pytest.mark.parametrize("R,K,stage", [(1, 1024, 0), (1, 8192, 1), (4, 16384, 2), (8, 4096, 0), (20, 8192, 9)])
+def test_matvec_scales_giving_up_leaves_no_load_in_flight(short_limit, R, K, stage):
+    """The producer goes on filling the ring after the scales' warp has left;
+    its wait for those loads ends with them, not with the limit."""
+    P, N = short_limit, 9000
+    x, p, s = _matvec(P, R, N, K, True, 44)
+    want = P.ops.matvec_w4(x, p, s)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
+    P.ops.selftest_matvec_stall(x, p, s, 1, stage)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 1
+    assert torch.equal(P.ops.matvec_w4(x, p, s), want)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
