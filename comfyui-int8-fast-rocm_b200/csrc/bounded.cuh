@@ -43,6 +43,7 @@ __device__ __forceinline__ bool wait_bounded_warp(uint64_t* bar, uint32_t parity
 // twice the limit at most: a role that owes the barrier arrivals may first
 // have to run out its own wait.
 __device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return;
   const uint64_t limit = 2 * *reinterpret_cast<volatile uint64_t*>(&g_tu_wait_limit_ns);
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {

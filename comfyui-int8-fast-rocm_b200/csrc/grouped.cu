@@ -69,6 +69,7 @@ struct GroupedParams {
   void* out;               // [R, N]
   int R, N, K;
   int early;               // the kernel before this one is gather_kernel
+  int stall;               // self-test: the stage, counted from 0, that a pair's producers leave out; else -1
 };
 
 struct Smem {  // behind the operand ring
@@ -258,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       tma_prefetch_desc(&tmW);
       for (int i = 0; i < BOXES; ++i) tma_prefetch_desc(&tmX.box[i]);
-      int stage = 0, e = 0;
+      int stage = 0, e = 0, fills = 0;
       uint32_t phase = 0;
       Armed armed;
       bool ok = true;
@@ -284,12 +285,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const CUtensorMap* tmx = &tmX.box[box_of(t)];
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
-          if (ahead > 0) --ahead;
-          else load_w(stage, t, kb);
-          const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
-          if constexpr (SL == 1) tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
-          else tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
-          armed.note(stage, phase);
+          if (fills++ != p.stall) {
+            if (ahead > 0) --ahead;
+            else load_w(stage, t, kb);
+            const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
+            if constexpr (SL == 1) tma_load_2d_pair(sX + stage * SLAB, tmx, fb, kb * BK, xrow);
+            else tma_load_3d_pair(sX + stage * SL * SLAB, tmx, fb, 0, xrow, kb * SL);
+            armed.note(stage, phase);
+          }
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -330,7 +333,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      if (*abort_flag && issued) {  // MMAs complete before TMEM is released
+      // MMAs complete before TMEM is released, also when the epilogue gives up
+      // after this loop has ended
+      if (issued) {
         umma_commit_pair(&s->drain, 0x1);
         wait_drain(&s->drain, 0);
       }
@@ -449,7 +454,7 @@ size_t grouped_workspace_bytes(int64_t R, int64_t K) { return gather_scale_offse
 
 int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
                    const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
-                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream) {
+                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall) {
   const int sms = device_sm_count();
   if (sms < 2) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
   if (a_rows != nullptr) {
@@ -471,7 +476,7 @@ int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8
     rc = encode_slab_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i, slabs);
   if (rc) return rc;
   const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K,
-                        a_rows != nullptr};
+                        a_rows != nullptr, stall};
   // tiles at most: every expert adds one partly filled row block to R / 256
   const int64_t tiles = (R / BT + (E < R ? E : R)) * ((N + 2 * BM - 1) / (2 * BM));
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);

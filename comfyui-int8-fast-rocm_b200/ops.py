@@ -934,6 +934,20 @@ def selftest_gemm_stall(a_q, a_scale, w_q, w_scale, stall_kb: int = 0) -> torch.
     return out
 
 
+def selftest_grouped_stall(a_q, a_scale, w_q, w_scale, offsets, which: int = 0, stage: int = 0) -> torch.Tensor:
+    """:func:`gemm_w8a8_grouped` (bf16 out, no gathered rows or bias, K a
+    multiple of 16) with stage ``stage`` of each CTA pair never loaded
+    (``which`` 0): the wait for it runs out and the kernel returns with error
+    bit 0 set.  Returns the (partly written) output."""
+    a_q, w_q = _aligned(a_q), _aligned(w_q)
+    R, K = a_q.shape
+    E, Nn, _ = w_q.shape
+    out = torch.empty((R, Nn), dtype=torch.bfloat16, device=a_q.device)
+    N.call("qlin_selftest_grouped_stall", a_q.data_ptr(), a_scale.data_ptr(), w_q.data_ptr(), w_scale.data_ptr(),
+           offsets.data_ptr(), E, out.data_ptr(), R, Nn, K, int(which), int(stage), _stream(a_q))
+    return out
+
+
 def selftest_matvec_stall(x, w_packed, w_scale, which: int = 0, stage: int = 0) -> torch.Tensor:
     """:func:`matvec_w4` of contiguous bf16 ``x`` without experts whose
     producer (``which`` 0: of the weights; 1: of group scales) never fills

@@ -113,6 +113,16 @@ QLIN_API int qlin_selftest_wait_timeout(int which, void* stream);
 QLIN_API int qlin_selftest_gemm_stall(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale,
                                       void* out, int64_t M, int64_t N, int64_t K, int64_t stall_kb, void* stream);
 
+/* Self-test of the grouped product's abort path: qlin_gemm_w8a8_grouped with
+ * bf16 output, without gathered rows or a bias.  which 0: both TMA producers
+ * of each CTA pair leave stage `stage` (counted from 0) unfilled, so that the
+ * MMA issuer's wait for it runs out after the limit: error bit 0 is set and
+ * the kernel returns with `out` partly written.  A stage that no pair reaches
+ * changes nothing. */
+QLIN_API int qlin_selftest_grouped_stall(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale,
+                                         const int32_t* offsets, int64_t E, void* out, int64_t R, int64_t N, int64_t K,
+                                         int which, int64_t stage, void* stream);
+
 /* Self-test of the 4-bit matrix-vector product's abort path: qlin_matvec_w4
  * of bf16 x [R, K] without experts, gathered rows or a bias, K <= 16384 and a
  * multiple of 32, 16-byte aligned weights.  which 0: the TMA producer of each

@@ -957,3 +957,14 @@ def test_matvec_stall_refusals(pkg):
     assert st(group=64) == unsup
     assert st(w=24) == st(ws=24) == align
     assert st(which=1, group=0) == st(which=2) == bad
+
+
+def test_grouped_stall_refusals(pkg):
+    N = pkg._native
+    lib = N.load()
+    bad, align = N.ERR_INVALID_ARG, N.ERR_ALIGNMENT
+    st = lambda a=16, E=2, R=4, Nn=8, K=32, which=0, stage=0, off=16: \
+        lib.qlin_selftest_grouped_stall(a, 16, 16, 16, off, E, 16, R, Nn, K, which, stage, None)
+    assert st(a=None) == st(E=0) == st(E=513) == st(R=0) == st(Nn=0) == st(K=0) == st(K=131072) == st(off=None) == bad
+    assert st(which=-1) == st(stage=-1) == st(E=512, Nn=2 ** 23) == bad
+    assert st(K=40) == st(a=24) == align

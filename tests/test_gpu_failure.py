@@ -115,3 +115,32 @@ def test_matvec_scales_giving_up_leaves_no_load_in_flight(short_limit, R, K, sta
     assert torch.equal(P.ops.matvec_w4(x, p, s), want)
     torch.cuda.synchronize()
     assert P.ops.device_error() == 0
+
+
+def _grouped(P, counts, N, K, seed=45):
+    g = torch.Generator().manual_seed(seed)
+    R, E = sum(counts), len(counts)
+    a = torch.randint(-127, 128, (R, K), generator=g).to(torch.int8).cuda()
+    w = torch.randint(-127, 128, (E, N, K), generator=g).to(torch.int8).cuda()
+    off = torch.tensor([0, *np.cumsum(counts)], dtype=torch.int32).cuda()
+    return a, torch.rand(R, 1, generator=g).cuda() * 1e-2, w, torch.rand(E, N, generator=g).cuda() * 1e-3, off
+
+
+GROUPED_STALLS = [([1], 200, 512, 1), ([300, 5, 700], 1000, 2048, 7), ([3, 0, 40], 600, 1328, 4),
+                  ([2000, 90] * 8, 2048, 1024, 13), ([2000, 90] * 8, 2048, 1024, 0)]
+
+
+@pytest.mark.parametrize("counts,N,K,stage", GROUPED_STALLS)
+def test_grouped_stall_aborts_and_recovers(short_limit, counts, N, K, stage):
+    P = short_limit
+    a, xs, w, ws, off = _grouped(P, counts, N, K)
+    want = P.ops.gemm_w8a8_grouped(a, xs, w, ws, off)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
+    P.ops.selftest_grouped_stall(a, xs, w, ws, off, 0, stage)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 1
+    assert torch.equal(P.ops.gemm_w8a8_grouped(a, xs, w, ws, off), want)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
+    _check_normal_gemm(P)
