@@ -195,14 +195,15 @@ QLIN_API int qlin_selftest_grouped_stall(const int8_t* a, const float* a_scale, 
   if (R <= 0 || N <= 0 || K <= 0 || K > 131056 || R > INT32_MAX - 256 || N > INT32_MAX - 256 || E * N > INT32_MAX - 256)
     return fail(QLIN_ERR_INVALID_ARG, "bad shape");
   if (K % 16) return fail(QLIN_ERR_ALIGNMENT, "K must be a multiple of 16");
-  if (which != 0) return fail(QLIN_ERR_INVALID_ARG, "which must be 0 (both producers)");
+  if (which < 0 || which > 2)
+    return fail(QLIN_ERR_INVALID_ARG, "which must be 0 (both producers), 1 (the leader's) or 2 (its peer's)");
   if (stage < 0 || stage > INT32_MAX) return fail(QLIN_ERR_INVALID_ARG, "stage out of range");
   if (!a || !a_scale || !w || !w_scale || !offsets || !out) return fail(QLIN_ERR_INVALID_ARG, "null pointer");
   if (!aligned16(a) || !aligned16(w) || !aligned16(out)) return fail(QLIN_ERR_ALIGNMENT, "operands must be 16-byte aligned");
   int rc = check_device();
   if (rc) return rc;
   return launch_grouped(a, a_scale, R, w, w_scale, offsets, E, nullptr, nullptr, out, DT_BF16, R, N, K, nullptr,
-                        static_cast<cudaStream_t>(stream), (int)stage);
+                        static_cast<cudaStream_t>(stream), (int)stage, which == 0 ? 2 : which - 1);
 }
 
 QLIN_API int qlin_selftest_matvec_stall(const void* x, const int8_t* w_packed, const float* w_scale, int group,

@@ -69,13 +69,16 @@ struct GroupedParams {
   void* out;               // [R, N]
   int R, N, K;
   int early;               // the kernel before this one is gather_kernel
-  int stall;               // self-test: the stage, counted from 0, that a pair's producers leave out; else -1
+  // Self-test: the stage, counted from 0, that both producers of a pair leave
+  // out (stall_rank 2), or before which that of one CTA waits in vain; else -1.
+  int stall, stall_rank;
 };
 
 struct Smem {  // behind the operand ring
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], drain;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], drain, never;
   uint32_t tmem_slot;
   int abort_flag;
+  int other_fills;                   // stages that the other CTA's producer filled, once its loop has ended; -1 before
   int ready[2];                      // whether an accumulator was complete in time: what all epilogue threads go by
   alignas(16) float xs[2][BT];       // activation scales of a tile's rows
   int begin[MAX_EXPERTS + 1];        // first row of each expert, ascending within [0, R]
@@ -111,6 +114,11 @@ __device__ __forceinline__ int box_of(const Tile& t) {
   int box = 0;
   while ((32 << box) < t.width) ++box;
   return box;
+}
+
+// *at = v in CTA `rank` of the cluster.
+__device__ __forceinline__ void store_cluster(const int* at, uint32_t rank, int v) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(at), rank)), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
@@ -226,7 +234,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       mbar_init(&s->tempty[b], 2 * EPI_WARPS);
     }
     mbar_init(&s->drain, 1);
+    mbar_init(&s->never, 1);
     *abort_flag = 0;
+    s->other_fills = -1;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -262,7 +272,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int stage = 0, e = 0, fills = 0;
       uint32_t phase = 0;
       Armed armed;
-      bool ok = true;
+      const int skip = p.stall_rank == 2 ? p.stall : -1, vain = p.stall_rank == (int)rank ? p.stall : -1;
+      // After a wait that ran out, the stages that the other producer filled:
+      // both end with as many, since the leader arms and awaits the loads of
+      // both, and no load may outlive the kernel.
+      int until = INT32_MAX;
       int ahead = 0;  // stages whose weights were asked for before the rows could be
       auto load_w = [&](int st, const Tile& t, int kb) {
         const uint32_t fb = mapa_shared(smem_u32(&s->full[st]), 0);
@@ -279,13 +293,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         pdl_wait();
       }
-      for (int tile = first; tile < num_tiles && ok; tile += step) {
+      for (int tile = first; tile < num_tiles && fills < until; tile += step) {
         const Tile t = locate(s, tile, e);
         const int xrow = t.row0 + (int)rank * (t.width >> 1);
         const CUtensorMap* tmx = &tmX.box[box_of(t)];
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
-          if (fills++ != p.stall) {
+          if (until == INT32_MAX && !(fills != vain ? wait_bounded(&s->empty[stage], phase ^ 1, abort_flag)
+                                                    : wait_bounded(&s->never, 0, abort_flag))) {
+            store_cluster(&s->other_fills, rank ^ 1, fills);
+            store_cluster(&s->abort_flag, rank ^ 1, 1);
+            until = max(fills, wait_value(&s->other_fills));
+          }
+          if (fills == until) break;
+          // (behind a wait that ran out: the other CTA's producer saw the stage
+          // empty, and one commit empties it in both)
+          if (fills++ != skip) {
             if (ahead > 0) --ahead;
             else load_w(stage, t, kb);
             const uint32_t fb = mapa_shared(smem_u32(&s->full[stage]), 0);
@@ -296,6 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
+      if (until == INT32_MAX) store_cluster(&s->other_fills, rank ^ 1, fills);
       // no load still writing shared memory at exit (both CTAs' loads are
       // counted by the leader; the peer waits for it at the last cluster barrier)
       if (leader) armed.drain(s->full);
@@ -454,7 +477,8 @@ size_t grouped_workspace_bytes(int64_t R, int64_t K) { return gather_scale_offse
 
 int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
                    const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
-                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall) {
+                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall,
+                   int stall_rank) {
   const int sms = device_sm_count();
   if (sms < 2) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
   if (a_rows != nullptr) {
@@ -476,7 +500,7 @@ int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8
     rc = encode_slab_tmap(&tx.box[i], a, (uint64_t)K, (uint64_t)R, BK, 16 << i, slabs);
   if (rc) return rc;
   const GroupedParams p{a_scale, w_scale, offsets, (int)E, bias, out, (int)R, (int)N, (int)K,
-                        a_rows != nullptr, stall};
+                        a_rows != nullptr, stall, stall_rank};
   // tiles at most: every expert adds one partly filled row block to R / 256
   const int64_t tiles = (R / BT + (E < R ? E : R)) * ((N + 2 * BM - 1) / (2 * BM));
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);

@@ -175,7 +175,8 @@ int launch_combine(int dt, const void* y, int64_t R, int64_t N, int64_t ldy, con
                    int64_t T, int top_k, const void* residual, int64_t ld_res, void* out, cudaStream_t stream);
 int launch_grouped(const int8_t* a, const float* a_scale, int64_t Ra, const int8_t* w, const float* w_scale,
                    const int32_t* offsets, int64_t E, const int32_t* a_rows, const void* bias, void* out, int out_dt,
-                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall = -1);
+                   int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall = -1,
+                   int stall_rank = -1);
 size_t grouped_workspace_bytes(int64_t R, int64_t K);  // of a gathered call
 int set_grouped_wait_limit(uint64_t ns);
 int read_grouped_error(cudaStream_t stream, uint32_t* bits);

@@ -937,8 +937,8 @@ def selftest_gemm_stall(a_q, a_scale, w_q, w_scale, stall_kb: int = 0) -> torch.
 def selftest_grouped_stall(a_q, a_scale, w_q, w_scale, offsets, which: int = 0, stage: int = 0) -> torch.Tensor:
     """:func:`gemm_w8a8_grouped` (bf16 out, no gathered rows or bias, K a
     multiple of 16) with stage ``stage`` of each CTA pair never loaded
-    (``which`` 0): the wait for it runs out and the kernel returns with error
-    bit 0 set.  Returns the (partly written) output."""
+    (``which`` 0), or loaded late by the leader (1) or its peer (2): the wait
+    for it runs out and the kernel returns with error bit 0 set.  Returns the (partly written) output."""
     a_q, w_q = _aligned(a_q), _aligned(w_q)
     R, K = a_q.shape
     E, Nn, _ = w_q.shape

@@ -117,8 +117,9 @@ QLIN_API int qlin_selftest_gemm_stall(const int8_t* a, const float* a_scale, con
  * bf16 output, without gathered rows or a bias.  which 0: both TMA producers
  * of each CTA pair leave stage `stage` (counted from 0) unfilled, so that the
  * MMA issuer's wait for it runs out after the limit: error bit 0 is set and
- * the kernel returns with `out` partly written.  A stage that no pair reaches
- * changes nothing. */
+ * the kernel returns with `out` partly written.  which 1 and 2: the producer
+ * of the pair's leader, or of its peer, waits in vain before that stage while
+ * the other goes on.  A stage that no pair reaches changes nothing. */
 QLIN_API int qlin_selftest_grouped_stall(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale,
                                          const int32_t* offsets, int64_t E, void* out, int64_t R, int64_t N, int64_t K,
                                          int which, int64_t stage, void* stream);

@@ -966,5 +966,5 @@ def test_grouped_stall_refusals(pkg):
     st = lambda a=16, E=2, R=4, Nn=8, K=32, which=0, stage=0, off=16: \
         lib.qlin_selftest_grouped_stall(a, 16, 16, 16, off, E, 16, R, Nn, K, which, stage, None)
     assert st(a=None) == st(E=0) == st(E=513) == st(R=0) == st(Nn=0) == st(K=0) == st(K=131072) == st(off=None) == bad
-    assert st(which=-1) == st(stage=-1) == st(E=512, Nn=2 ** 23) == bad
+    assert st(which=-1) == st(which=3) == st(stage=-1) == st(E=512, Nn=2 ** 23) == bad
     assert st(K=40) == st(a=24) == align

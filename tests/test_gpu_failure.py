@@ -144,3 +144,21 @@ def test_grouped_stall_aborts_and_recovers(short_limit, counts, N, K, stage):
     torch.cuda.synchronize()
     assert P.ops.device_error() == 0
     _check_normal_gemm(P)
+
+
+@pytest.mark.parametrize("which", [1, 2])
+@pytest.mark.parametrize("counts,N,K,stage", GROUPED_STALLS)
+def test_grouped_one_producer_giving_up_leaves_no_load_in_flight(short_limit, counts, N, K, stage, which):
+    """The other producer of the pair goes on filling the ring; both end with
+    as many stages filled, and the leader awaits all of them."""
+    P = short_limit
+    a, xs, w, ws, off = _grouped(P, counts, N, K, 46)
+    want = P.ops.gemm_w8a8_grouped(a, xs, w, ws, off)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
+    P.ops.selftest_grouped_stall(a, xs, w, ws, off, which, stage)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 1
+    assert torch.equal(P.ops.gemm_w8a8_grouped(a, xs, w, ws, off), want)
+    torch.cuda.synchronize()
+    assert P.ops.device_error() == 0
