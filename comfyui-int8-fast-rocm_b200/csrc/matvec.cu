@@ -64,6 +64,7 @@ constexpr int SMEM = 227 * 1024;
 struct MatvecParams {
   const void* x;
   int64_t Rx, ldx;
+  int64_t Rd;             // rows of digits: of the source rows, or of the result rows where they are fewer
   const uint8_t* w;       // [E, N, K / 2]
   const void* scale;      // [E, N, groups]
   int scale_bf16;
@@ -86,8 +87,8 @@ struct MatvecParams {
   int stall_weights;      // self-test: the stage, counted from 0, that a block's producer leaves out; else -1
   int stall_scales;       // and the one at which the scales' warp waits in vain
   // of split_kernel, in the caller's workspace
-  int8_t* digits;         // [Rx, blocks, half, digit, lane t, 16]
-  float* exps;            // [Rx, epitch] 2^e, negative where the row has infinities or NaN
+  int8_t* digits;         // [Rd, blocks, half, digit, lane t, 16]
+  float* exps;            // [Rd, epitch] 2^e, negative where the row has infinities or NaN
   int epitch;             // blocks rounded up to 4
 };
 
@@ -101,6 +102,12 @@ __device__ __forceinline__ float scale_at(const MatvecParams& p, int64_t i) {
 __device__ __forceinline__ int64_t source_row(const MatvecParams& p, int r) {
   const int64_t src = p.x_rows != nullptr ? (int64_t)p.x_rows[r] : r;
   return src >= 0 && src < p.Rx ? src : -1;
+}
+
+// where its digits are, or -1 as above
+__device__ __forceinline__ int64_t digit_row(const MatvecParams& p, int r) {
+  const int64_t src = source_row(p, r);
+  return src < 0 || p.Rd == p.Rx ? src : r;
 }
 
 // ---------------------------------------------------------------------------
@@ -186,11 +193,11 @@ __global__ void __launch_bounds__(1024) split_kernel(MatvecParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.x, src = p.Rd == p.Rx ? r : source_row(p, (int)r);
   bool odd = false;
   for (int b = warp; b < p.blocks; b += blockDim.x >> 5) {
     float v[1][4];
-    load_x4<DT>(p, r, b, lane, v[0]);
+    load_x4<DT>(p, src, b, lane, v[0]);
     odd |= make_digits<1>(v, lane, {p.digits + (r * p.blocks + b) * (4 * KB)}, {p.exps + r * p.epitch + b}) != 0;
   }
   if (__syncthreads_or(odd))
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       bool ok = true;
       if (lane == 0 && loads > 0) ok = wait_bounded(&s->xempty, (loads - 1) & 1, abort_flag);
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
-      const int64_t src = lane < it.rows ? source_row(p, it.r0 + lane) : -1;
+      const int64_t src = lane < it.rows ? digit_row(p, it.r0 + lane) : -1;
       const uint32_t live = __ballot_sync(0xffffffffu, src >= 0);
       if (lane < it.rows && src < 0)  // a row of zeros: whatever its digits are
         for (int i = 0; i < p.epitch; ++i) xexp[lane * p.epitch + i] = 0.0f;
@@ -761,8 +768,8 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
     int64_t src[CB], sum_src[CB];  // the rows whose digits this lane reads, whose sums it gets
 #pragma unroll
     for (int c = 0; c < CB; ++c) {
-      src[c] = source_row(p, r0 + min(2 * c + (g >> 2), rows - 1));
-      sum_src[c] = source_row(p, r0 + min(2 * c + (t >> 1), rows - 1));
+      src[c] = digit_row(p, r0 + min(2 * c + (g >> 2), rows - 1));
+      sum_src[c] = digit_row(p, r0 + min(2 * c + (t >> 1), rows - 1));
     }
     float sum[CB][2];
 #pragma unroll
@@ -821,8 +828,8 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
       float v = 0.0f;
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) v += s_part[k][threadIdx.x & 15][r];
-      const int64_t at = (int64_t)e * p.N + n, from = source_row(p, r0 + r);
-      if (from >= 0 && p.exps[from * p.epitch] < 0.0f) v += odd_terms<DT>(p, from, at);
+      const int64_t at = (int64_t)e * p.N + n, from = digit_row(p, r0 + r);
+      if (from >= 0 && p.exps[from * p.epitch] < 0.0f) v += odd_terms<DT>(p, source_row(p, r0 + r), at);
       if constexpr (!GROUPS) v *= scale_at(p, at);
       if (p.bias != nullptr) v += Elem<DT>::to_f(reinterpret_cast<const T*>(p.bias)[at]);
       reinterpret_cast<T*>(p.out)[(int64_t)(r0 + r) * p.N + n] = Elem<DT>::from_f(v);
@@ -909,7 +916,7 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   p.early = !p.own_digits && p.Rx > 0;
   if (p.early) {
     const int threads = 32 * (p.blocks < 32 ? p.blocks : 32);
-    e = launch_pdl(split_kernel<DT>, dim3((unsigned)p.Rx), dim3(threads), 0, stream, p);
+    e = launch_pdl(split_kernel<DT>, dim3((unsigned)p.Rd), dim3(threads), 0, stream, p);
     if (e != cudaSuccess) return cuda_fail(e, "matvec_w4 split launch");
   }
   if (!fast) {
@@ -937,15 +944,16 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
 bool aligned_weights(const uint8_t* w, int64_t K) { return K % 32 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0; }
 
 struct Workspace {
-  int64_t blocks, epitch;
+  int64_t rows, blocks, epitch;
   size_t exps, bytes;
 };
-Workspace workspace_layout(int64_t Rx, int64_t K) {
+Workspace workspace_layout(int64_t R, int64_t Rx, int64_t K) {
   Workspace w;
+  w.rows = R < Rx ? R : Rx;
   w.blocks = (K + KB - 1) / KB;
   w.epitch = (w.blocks + 3) & ~int64_t(3);
-  w.exps = (size_t)(Rx * w.blocks * (4 * KB));
-  w.bytes = w.exps + (size_t)(Rx * w.epitch) * sizeof(float);
+  w.exps = (size_t)(w.rows * w.blocks * (4 * KB));
+  w.bytes = w.exps + (size_t)(w.rows * w.epitch) * sizeof(float);
   return w;
 }
 
@@ -953,7 +961,7 @@ Workspace workspace_layout(int64_t Rx, int64_t K) {
 
 size_t matvec_workspace_bytes(const uint8_t* w, bool experts, int64_t R, int64_t Rx, int64_t N, int64_t K) {
   if (aligned_weights(w, K) && makes_own_digits(experts, R, K)) return 0;
-  return workspace_layout(Rx, K).bytes;
+  return workspace_layout(R, Rx, K).bytes;
 }
 
 int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8_t* w, const void* scale, int scale_dt,
@@ -961,10 +969,11 @@ int launch_matvec_w4(int dt, const void* x, int64_t Rx, int64_t ldx, const uint8
                      int64_t R, int64_t N, int64_t K, void* workspace, cudaStream_t stream, int stall_weights,
                      int stall_scales) {
   if (device_sm_count() < 1) return fail(QLIN_ERR_NO_DEVICE, "no CUDA device");
-  const Workspace l = workspace_layout(Rx, K);
+  const Workspace l = workspace_layout(R, Rx, K);
   MatvecParams p{};
   p.x = x;
   p.Rx = Rx;
+  p.Rd = l.rows;
   p.ldx = ldx;
   p.w = w;
   p.scale = scale;

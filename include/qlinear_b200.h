@@ -507,7 +507,8 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
  * once for each 2 to 8 rows of an expert, so many rows belong to the GEMMs.
  * workspace: qlin_matvec_w4_workspace bytes of device memory for these
  * arguments, 16-byte aligned, used within the call only (NULL when that is 0:
- * small calls without offsets, no rows).  out is 16-byte aligned; K % 32
+ * small calls without offsets, no rows); it goes by the source rows or the
+ * result rows, whichever are fewer.  out is 16-byte aligned; K % 32
  * == 0 and 16-byte aligned weights are read fastest. */
 QLIN_API int qlin_matvec_w4_workspace(const int8_t* w_packed, int has_offsets, int64_t R, int64_t Rx, int64_t N,
                                       int64_t K, uint64_t* bytes);

@@ -968,3 +968,40 @@ def test_grouped_stall_refusals(pkg):
     assert st(a=None) == st(E=0) == st(E=513) == st(R=0) == st(Nn=0) == st(K=0) == st(K=131072) == st(off=None) == bad
     assert st(which=-1) == st(which=3) == st(stage=-1) == st(E=512, Nn=2 ** 23) == bad
     assert st(K=40) == st(a=24) == align
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+def test_matvec_workspace_goes_by_the_fewer_rows(pkg, aligned):
+    """Few rows gathered out of a long x need no more room than those rows by themselves."""
+    import ctypes
+    lib, n = pkg._native.load(), ctypes.c_uint64(0)
+
+    def room(R, Rx, K=4096):
+        assert lib.qlin_matvec_w4_workspace(16 if aligned else 17, 1, R, Rx, 8, K, ctypes.addressof(n)) == 0
+        return n.value
+
+    assert 0 < room(8, 65536) == room(8, 8)
+    assert room(65536, 8) == room(8, 8)
+    assert room(0, 100) == room(100, 0) == 0
+
+
+@on_gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("K,groups", [(256, True), (2048, False), (258, False)])  # 258: the kernel for any depth
+@pytest.mark.parametrize("E", [None, 5])
+def test_matvec_few_rows_of_a_long_x(pkg, dt, K, groups, E):
+    """The same bits as for those rows laid out one after another."""
+    Rx, R = 700, 23
+    x, p, s, b = matvec_inputs(29 + K, Rx, E, 70, K, groups, dt, True)
+    x[5, 3], x[6, 7] = math.inf, math.nan
+    rows = torch.randint(0, Rx, (R,), generator=gen(10)).to(torch.int32)
+    rows[:6] = torch.tensor([5, 699, -1, 6, Rx, 699])
+    offsets = None if E is None else [0, 1, 9, 9, 21, 22]
+    got = run_matvec(pkg, x, p, s, b, offsets, rows)
+    inside = (rows >= 0) & (rows < Rx)
+    laid = torch.where(inside[:, None], x[rows.clamp(0, Rx - 1).long()], torch.zeros((), dtype=x.dtype))
+    assert torch.equal(got.nan_to_num(nan=7.0), run_matvec(pkg, laid, p, s, b, offsets).nan_to_num(nan=7.0))
+    good = torch.ones(R, dtype=torch.bool)
+    good[[0, 3]] = False
+    y, mag = matvec_ref(x.nan_to_num(0, 0, 0), p, s, b, offsets, rows)
+    assert_matvec(got[good.cuda()], y[good], mag[good], K)
