@@ -36,7 +36,9 @@ def _tokens(x: Tensor, logits: Tensor, residual):
     l2 = logits.reshape(-1, logits.shape[-1])
     if l2.shape[0] != x2.shape[0]:
         raise ValueError(f"{x2.shape[0]} tokens but {l2.shape[0]} rows of logits")
-    return x2, l2, None if residual is None else residual.reshape(x2.shape[0], -1)
+    if residual is not None:  # (-1 stands for any number where there are no tokens)
+        residual = residual.reshape(x2.shape[0], -1 if x2.shape[0] else residual.shape[-1])
+    return x2, l2, residual
 
 
 @torch.no_grad()

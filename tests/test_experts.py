@@ -1005,3 +1005,31 @@ def test_matvec_few_rows_of_a_long_x(pkg, dt, K, groups, E):
     good[[0, 3]] = False
     y, mag = matvec_ref(x.nan_to_num(0, 0, 0), p, s, b, offsets, rows)
     assert_matvec(got[good.cuda()], y[good], mag[good], K)
+
+
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (3,), (2, 3)])
+def test_feed_forward_tokens_and_residual(pkg, lead):
+    """Tokens, logits and residual as rows, also where there are none."""
+    x, logits, res = torch.zeros(*lead, 32), torch.zeros(*lead, 4), torch.zeros(*lead, 24)
+    T = math.prod(lead)
+    x2, l2, r2 = pkg.experts._tokens(x, logits, res)
+    assert (x2.shape, l2.shape, r2.shape) == ((T, 32), (T, 4), (T, 24))
+    assert pkg.experts._tokens(x, logits, None)[2] is None
+
+
+@on_gpu
+@pytest.mark.parametrize("lead", [(0,), (2, 0)])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rot", [None, ("regular", 64)])
+def test_feed_forward_without_tokens(pkg, lead, residual, rot):
+    E, K, F = 3, 128, 64
+    X, bf = pkg.experts, dict(dtype=torch.bfloat16, device="cuda")
+    x, logits = torch.zeros(*lead, K, **bf), torch.zeros(*lead, E, **bf)
+    res = torch.zeros(*lead, K, **bf) if residual else None
+    up, down = randn(160, E, 2 * F, K).cuda(), randn(161, E, K, F).cuda()
+    y = X.int8_forward_experts(x, logits, *X.quantize_experts_int8(up, rot), *X.quantize_experts_int8(down, rot), 2,
+                               residual=res, rot=rot, down_rot=rot)
+    assert (y.shape, y.dtype) == (x.shape, x.dtype)
+    y = X.w4_forward_experts(x, logits, *X.quantize_experts_int4(up, rot), *X.quantize_experts_int4(down, rot), 2,
+                             residual=res, rot=rot, down_rot=rot)
+    assert (y.shape, y.dtype) == (x.shape, x.dtype)
