@@ -1033,3 +1033,58 @@ def test_feed_forward_without_tokens(pkg, lead, residual, rot):
     y = X.w4_forward_experts(x, logits, *X.quantize_experts_int4(up, rot), *X.quantize_experts_int4(down, rot), 2,
                              residual=res, rot=rot, down_rot=rot)
     assert (y.shape, y.dtype) == (x.shape, x.dtype)
+
+
+def assert_matvec_closely(got, x, p, s, bias=None, offsets=None, rows=None):
+    """What the digits and float32 steps of the kernels may do.  Per 128 k: x
+    as integers in units of 2^(e - 29), e the exponent of their largest, each
+    off by half a unit at most; the digits' integer sums are exact, and their
+    two halves (whose magnitudes add up to the terms' and less than 2^-12 of
+    the largest x times the weights) each become a float32 and meet the scale,
+    two steps.  Then a multiply-add for each 128 k, the halves' sum, eight
+    warps' sums, the scale of a row and the bias: K / 128 + 13 steps of 2^-24
+    of the magnitude; last, half a step of the result's dtype."""
+    dt, K = got.dtype, x.shape[1]
+    y, mag = matvec_ref(x, p, s, bias, offsets, rows)
+    q = unpack(p).abs()
+    blocks = -(-K // 128)
+    pad = blocks * 128 - K
+    big = torch.nn.functional.pad(x.double().abs(), (0, pad)).reshape(-1, blocks, 128).amax(-1)
+    e = torch.where(big > 0, torch.frexp(big).exponent - 1, -126).clamp_min(-126)  # 2^e <= big < 2^(e + 1)
+    qs = torch.nn.functional.pad(q, (0, pad)).reshape(*q.shape[:-1], blocks, 128).sum(-1)
+    qs = qs * (s.double() if s.dim() == p.dim() and s.shape[-1] != 1 else s.double().reshape(*p.shape[:-1], 1))
+    src = torch.arange(x.shape[0]) if rows is None else rows.long()
+    inside = (src >= 0) & (src < x.shape[0])
+    unit = torch.where(inside[:, None], torch.exp2((e - 30).double())[src.clamp(0, x.shape[0] - 1)], 0.0)
+    off = torch.zeros_like(y)
+    for i, (b, t) in enumerate([(0, len(src))] if offsets is None else spans(offsets, len(src))):
+        off[b:t] = unit[b:t] @ (qs if offsets is None else qs[i]).T
+    tol = off * 1.01 + (K / 128 + 13) * U * 1.001 * (mag + off * 2 ** 18) + torch.finfo(dt).eps / 2 * 1.001 * y.abs() + \
+        torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    bad = ((got.cpu().double() - y).abs() > tol).sum().item()
+    assert bad == 0, f"{bad} of {y.numel()} values off"
+
+
+@on_gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("M,Nn,K,groups", [
+    (1, 300, 128, True), (1, 2048, 8192, True), (2, 129, 4224, False), (3, 200, 2048, True), (4, 100, 16384, True),
+    (8, 70, 1440, False), (9, 640, 1024, True), (33, 70, 2048, True),
+    (1, 33, 34, False), (3, 100, 258, False), (7, 50, 20002, False), (2, 40, 33408, True)])  # the kernel for any depth
+def test_matvec_closely(pkg, dt, M, Nn, K, groups):
+    x, p, s, b = matvec_inputs(30 + M + K, M, None, Nn, K, groups, dt, True)
+    assert_matvec_closely(run_matvec(pkg, x, p, s, b), x, p, s, b)
+
+
+@on_gpu
+@pytest.mark.parametrize("K,groups", [(384, True), (416, False), (386, False)])  # 386: the kernel for any depth
+@pytest.mark.parametrize("counts", [[1], [0, 3, 9, 1]])
+def test_matvec_experts_closely_with_a_large_value_under_zero_weights(pkg, K, groups, counts):
+    """A value 2^14 and more above the others sets the unit of its 128 k where its own weight is 0."""
+    R, E = sum(counts), len(counts)
+    x, p, s, b = matvec_inputs(31 + K, R, E, 60, K, groups, "f32", True)
+    x[:, 130] = 2.0 ** 17
+    p[:, :, 65] &= -16  # the low nibble of k 130
+    rows = torch.randint(-1, R + 1, (R,), generator=gen(11)).to(torch.int32)
+    for r in (None, rows):
+        assert_matvec_closely(run_matvec(pkg, x, p, s, b, cum(counts), r), x, p, s, b, cum(counts), r)
