@@ -421,8 +421,10 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
       const int64_t src = lane < it.rows ? digit_row(p, it.r0 + lane) : -1;
       const uint32_t live = __ballot_sync(0xffffffffu, src >= 0);
-      if (lane < it.rows && src < 0)  // a row of zeros: whatever its digits are
+      if (lane < it.rows && src < 0) {  // a row of zeros: whatever its digits are
         for (int i = 0; i < p.epitch; ++i) xexp[lane * p.epitch + i] = 0.0f;
+        fence_proxy_async_smem();  // a later pass's bulk copy writes here
+      }
       __syncwarp();
       const uint32_t dbytes = (uint32_t)p.blocks * (4 * KB), ebytes = (uint32_t)p.epitch * 4;
       if (lane == 0) mbar_arrive_expect_tx(&s->xfull, (uint32_t)__popc(live) * (dbytes + ebytes));

@@ -1088,3 +1088,18 @@ def test_matvec_experts_closely_with_a_large_value_under_zero_weights(pkg, K, gr
     rows = torch.randint(-1, R + 1, (R,), generator=gen(11)).to(torch.int32)
     for r in (None, rows):
         assert_matvec_closely(run_matvec(pkg, x, p, s, b, cum(counts), r), x, p, s, b, cum(counts), r)
+
+
+@on_gpu
+@pytest.mark.parametrize("M", [40, 200])
+def test_matvec_rows_of_zeros_and_others_in_turn(pkg, M):
+    """A row of zeros and a row of x at the same place of one pass after another."""
+    x, p, s, b = matvec_inputs(32, 9, None, 4500, 2048, True, "bf16", True)
+    rows = torch.randint(0, 9, (M,), generator=gen(12)).to(torch.int32)
+    rows[torch.arange(M) // 8 % 2 == 0] = -1
+    rows[torch.arange(M) % 5 == 0] = 9
+    got = run_matvec(pkg, x, p, s, b, None, rows).cpu()
+    at = torch.arange(0, 4500, 31)
+    inside = (rows >= 0) & (rows < 9)
+    assert torch.equal(got[~inside], b[None].expand(int((~inside).sum()), -1))
+    assert_matvec_closely(got[:, at], x, p[at], s[at], b[at], None, rows)
