@@ -15,18 +15,19 @@
 //                  integers X = x * 2^(29 - e), e the exponent of the largest
 //                  of them, each in four signed base-256 digits.  A value down
 //                  to 2^-6 (float32), 2^-19 (f16) or 2^-22 (bf16) of the
-//                  largest is exact, a smaller one off by 2^-30 of it at most,
-//                  less than a float32 sum of them loses;
+//                  largest is exact, a smaller one off by 2^-30 of the largest
+//                  at most: less than a float32 sum of the 128 loses where the
+//                  largest has a weight, and lost where its weight is 0;
 //   matvec_kernel  mma.sync m16n8k32 (int8): 16 weight rows times 8 columns,
 //                  the four digits of two rows.  The int32 sums of a block of
-//                  128 are exact; digits and scales meet once a block in
-//                  float32.
+//                  128 are exact; their upper and lower two digits become a
+//                  float32 each, meet the scale and are added up in float32.
 //
-// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 15.0 us: about 5 us
-// of launches and latency, then 5.4 TB/s (N 98304 5.5 TB/s in all; a copy of the
+// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 15.7 us: about 5 us
+// of launches and latency, then 5.2 TB/s (N 98304 5.5 TB/s in all; a copy of the
 // kernel that only loads 5.9).  With more rows the multiplying warps do, two to a
-// scheduler that issue an instruction every four clocks or so (4 rows 18.4 us, 8
-// rows 24.0); 16 of them, with half a stage each, are no faster, since what a
+// scheduler that issue an instruction every four clocks or so (4 rows 18.9 us, 8
+// rows 25.0); 16 of them, with half a stage each, are no faster, since what a
 // warp does once a stage and a tile doubles.
 //
 // matvec_kernel is persistent, a block of threads a SM.  One warp brings the
@@ -841,9 +842,12 @@ __global__ void __launch_bounds__(32 * WARPS) matvec_any_kernel(MatvecParams p) 
 }
 
 // Few values: every block of threads makes the digits itself, which saves a
-// launch and a workspace, 4 of 19 us of a call.  On the device one row of K 4096
-// takes as long as with split_kernel (N 24576: 15.0 us, 14.7), two rows 0.3 to
-// 1.2 us longer, 4 rows 3 to 4 us: more than the call saves in a graph.
+// launch and a workspace: a call takes 12.8 us instead of 17.4.  On the device
+// (bf16, us; with split_kernel) one row gains: N 24576, K 4096 15.5 (16.3), N
+// 8192, K 8192 11.4 (11.8); two rows are even: N 8192, K 4096 9.5 (9.3); more
+// rows lose, which a replayed graph pays: 4 of N 8192, K 2048 9.7 (8.9), 5 of N
+// 1111, K 1440 8.8 (7.2), 8 of N 8192, K 1024 10.9 (9.5).  With more values, 4
+// rows of K 4096, the device loses 3 to 4 us, nearly what the call gains.
 bool makes_own_digits(bool experts, int64_t R, int64_t K) { return !experts && R <= 8 && R * K <= 8192; }
 
 template <int CB>
@@ -936,7 +940,11 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   // on the device only): more columns than rows cost more than a second pass
   // over an expert's weights, which L2 then holds (32 rows of 8 experts, N
   // 8192, K 4096: 43 us with 4 rows a pass, 47 with 8; 16 rows 32 us with 4 rows
-  // a pass, 34 with 2; 4 rows of one weight, N 24576: 19 and 24).
+  // a pass, 34 with 2; 4 rows of one weight, N 24576: 19 and 24).  launch_cfg may
+  // find room for fewer rows than the instance has columns for (K 8192 4 of 8,
+  // 11008 3, 14336 2, above about 20,000 one), and the pass then costs what all
+  // columns cost: N 4096, 4 rows 10.4 us at K 8192, 21.0 at K 11008; 8 rows 19.1
+  // and 32.1.
   const int64_t sets = p.offsets == nullptr ? 1 : p.E;
   if (p.offsets == nullptr ? p.R <= 2 : p.R < 2 * sets) return launch_cb<DT, 1>(p, stream);
   if (p.R < 5 * sets) return launch_cb<DT, 2>(p, stream);

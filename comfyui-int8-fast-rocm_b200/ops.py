@@ -782,7 +782,8 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, pos: torch.Tensor, r
 def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=None, out_dtype=torch.bfloat16):
     """W8A8 linear of rows sorted by expert: rows ``offsets[e] ..
     offsets[e + 1]`` of the result are :func:`gemm_w8a8` of those rows with
-    expert e's weight, bit for bit.  ``a_q`` [Ra, K] int8, ``a_scale`` [Ra]
+    expert e's weight, bit for bit (with a 16-bit result also rounded before
+    the bias is added).  ``a_q`` [Ra, K] int8, ``a_scale`` [Ra]
     (or [Ra, 1]), ``w_q`` [E, N, K] int8, ``w_scale`` [E, N], ``offsets``
     int32 [E + 1] on the device, ``bias`` [E, N].
 
@@ -832,8 +833,10 @@ def gemm_w8a8_grouped(a_q, a_scale, w_q, w_scale, offsets, a_rows=None, bias=Non
 
 def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     """Linear of few rows with packed 4-bit weights, the activations not
-    quantised: ``y = dt(x @ (q * scale).T + bias)`` with exact sums of each
-    128 k, float32 sums of those, and one rounding (see qlin_matvec_w4).
+    quantised: ``y = dt(x @ (q * scale).T + bias)`` with integer sums of each
+    128 k (x in units of 2^-30 to 2^-29 of their largest), float32 sums of
+    those, and one rounding (see qlin_matvec_w4).  With one scale a row it
+    comes last: a sum of |x * q| above float32's largest overflows.
     ``x`` [Rx, K] (bf16/f16/f32, row-strided views are read in place),
     ``w_packed`` [N, K/2] and ``w_scale`` [N] (or [N, 1]) or [N, K/128],
     float32 or bfloat16, as :func:`quant_weight_int4` returns them; ``bias``
@@ -845,7 +848,8 @@ def matvec_w4(x, w_packed, w_scale, bias=None, offsets=None, x_rows=None):
     :func:`gemm_w8a8_grouped`).  ``x_rows`` [R] gathers: result row r takes
     row ``x_rows[r]`` of ``x`` (an index outside [0, Rx) is a row of zeros).
 
-    The weights are read once for each 2 to 8 rows of an expert; many rows are
+    The weights are read once for each pass of up to 8 rows of an expert (4 at
+    K 8192, 2 at K 16384, one above about 20000); many rows are
     :func:`gemm_w4_g128`'s and :func:`gemm_w8a8_grouped`'s work."""
     if w_packed.dtype != torch.int8:
         raise TypeError("packed int4 weights are int8 tensors")

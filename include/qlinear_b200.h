@@ -477,7 +477,8 @@ QLIN_API int qlin_combine_experts(const void* y, int dtype, int64_t R, int64_t N
 
 /* W8A8 linear of rows sorted by expert: for the rows r of expert e,
  *   out[r] = qlin_gemm_w8a8(a[src(r)], a_scale[src(r)], w[e], w_scale[e], bias[e])
- * bit for bit (QLIN_WSCALE_ROW), src(r) = a_rows ? a_rows[r] : r.  a [Ra, K],
+ * bit for bit (QLIN_WSCALE_ROW; with a bias and a 16-bit out it rounds before
+ * and after the bias too), src(r) = a_rows ? a_rows[r] : r.  a [Ra, K],
  * w [E, N, K], w_scale [E, N], bias [E, N] in out_dtype or NULL, out [R, N];
  * R = Ra without a_rows.  Rows of no expert become 0; a source row outside
  * [0, Ra) counts as a row of zeros.  K % 16 == 0, K <= 131056 (the int32 sum
@@ -496,15 +497,21 @@ QLIN_API int qlin_gemm_w8a8_grouped(const int8_t* a, const float* a_scale, int64
  * with one rounding; q signed nibbles [N, K/2] (low nibble = even k), group
  * 128 (K % 128 == 0) or 0 (one scale a row, any even K), the layouts of
  * qlin_quant_weight_int4; w_scale F32 or BF16.  x [Rx, K] (row stride ldx)
- * and bias [N] in x_dtype, out [R, N] in x_dtype.  Each 128 k are summed
- * exactly, with x as 32-bit integers in units of 2^-30 of their largest
- * (which 16-bit values are, exactly, down to 2^-19 of it); the sums of the
- * 128 are scaled and added in float32.
+ * and bias [N] in x_dtype, out [R, N] in x_dtype.  Of each 128 k, x becomes
+ * 32-bit integers in units of 2^(e - 29), 2^e the power of two at or below
+ * their largest (exact for 16-bit values down to 2^-19 of it, else off by half
+ * a unit, also where the largest meets a zero weight); their products are
+ * summed exactly, in two halves that become float32 numbers, and those are
+ * scaled and added in float32.  With one scale a row it comes last, as above:
+ * where sum |x * q| exceeds float32's largest (one x of 4.3e37 is enough) the
+ * result is not finite, whatever the scale.
  * offsets NULL: E == 1, all rows use the one weight.  Otherwise w_packed
  * [E, N, K/2], w_scale [E, N, G] and bias [E, N], rows sorted by expert; rows
  * of no expert become 0.  src(r) = x_rows ? x_rows[r] : r; a source row
  * outside [0, Rx) counts as a row of zeros.  Any R works; the weights are read
- * once for each 2 to 8 rows of an expert, so many rows belong to the GEMMs.
+ * once for each pass of up to 8 rows of an expert (of those whose digits, 4 K
+ * bytes a row, fit in shared memory: 8 up to K 4096, 4 at 8192, 2 at 16384,
+ * one above about 20000), so many rows belong to the GEMMs.
  * workspace: qlin_matvec_w4_workspace bytes of device memory for these
  * arguments, 16-byte aligned, used within the call only (NULL when that is 0:
  * small calls without offsets, no rows); it goes by the source rows or the
