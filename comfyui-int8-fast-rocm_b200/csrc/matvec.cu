@@ -23,11 +23,11 @@
 //                  128 are exact; their upper and lower two digits become a
 //                  float32 each, meet the scale and are added up in float32.
 //
-// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 15.7 us: about 5 us
-// of launches and latency, then 5.2 TB/s (N 98304 5.5 TB/s in all; a copy of the
+// What bounds it: one row, N 24576, K 4096 (53.6 MB) takes 15.0 us: about 5 us
+// of launches and latency, then 5.4 TB/s (N 98304 5.5 TB/s in all; a copy of the
 // kernel that only loads 5.9).  With more rows the multiplying warps do, two to a
-// scheduler that issue an instruction every four clocks or so (4 rows 18.9 us, 8
-// rows 25.0); 16 of them, with half a stage each, are no faster, since what a
+// scheduler that issue an instruction every four clocks or so (4 rows 18.4 us, 8
+// rows 24.9); 16 of them, with half a stage each, are no faster, since what a
 // warp does once a stage and a tile doubles.
 //
 // matvec_kernel is persistent, a block of threads a SM.  One warp brings the
@@ -593,16 +593,20 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
     }
     int stage = 0, now = -1, buf = 0;
     uint32_t phase = 0, loads = 0, pphase = 0;
-    bool ok = true;
+    // 0 once a wait of this lane ran out: it then goes on with whatever the
+    // stages hold, so that all lanes meet below, and the warp's verdict is taken
+    // once an item.  Bit 0: lane 0, which arrives for the warp.  (8 rows of N
+    // 24576, K 4096: 24.8 us, with a vote a stage 26.0.)
+    int arrives = lane == 0 ? 3 : 2;
     Item it;
-    for (it.start(p, s); it.left > 0 && ok; it.next(p, s)) {
+    for (it.start(p, s); it.left > 0; it.next(p, s)) {
       if (it.pass != now) {
         if (now >= 0) {  // this warp is done with the digits of the pass before
           __syncwarp();
           if (lane == 0) mbar_arrive(&s->xempty);
         }
         now = it.pass;
-        ok = wait_bounded_warp(&s->xfull, loads & 1, abort_flag);
+        if (!wait_bounded(&s->xfull, loads & 1, abort_flag)) arrives = 0;
         ++loads;
       }
       const uint8_t* xd[CB];
@@ -617,13 +621,10 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int c = 0; c < CB; ++c) sum[i][c][0] = sum[i][c][1] = 0.0f;
-      // A lane whose wait ran out goes on with whatever the stage holds, so that
-      // all lanes meet below; the warp's verdict is taken once an item (8 rows of
-      // N 24576, K 4096: 24.5 us, with a vote a stage 26.0).
 #pragma unroll 1
       for (int st = 0; st < steps; ++st) {
         const int b0 = st * 2 * slabs + bi;
-        if (ok) ok = wait_bounded(&s->full[stage], phase, abort_flag);
+        if (!wait_bounded(&s->full[stage], phase, abort_flag)) arrives = 0;
 #pragma unroll
         for (int k = 0; k < BLK; ++k) {
           // Behind K the weights are 0, and the last block's digits and exponent
@@ -691,12 +692,11 @@ __global__ void __launch_bounds__(THREADS, 1) matvec_kernel(const __grid_constan
           }
         }
         __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(&s->empty[stage]);
+        if (arrives & 1) mbar_arrive(&s->empty[stage]);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
-      if (ok) ok = wait_bounded(&s->pempty[buf], pphase ^ 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!wait_bounded(&s->pempty[buf], pphase ^ 1, abort_flag)) arrives = 0;
+      if (!__all_sync(0xffffffffu, arrives)) break;
       float* to = part + (buf * WARPS + warp) * PART;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -943,8 +943,8 @@ int launch_dt(MatvecParams p, bool aligned, cudaStream_t stream) {
   // a pass, 34 with 2; 4 rows of one weight, N 24576: 19 and 24).  launch_cfg may
   // find room for fewer rows than the instance has columns for (K 8192 4 of 8,
   // 11008 3, 14336 2, above about 20,000 one), and the pass then costs what all
-  // columns cost: N 4096, 4 rows 10.4 us at K 8192, 21.0 at K 11008; 8 rows 19.1
-  // and 32.1.
+  // columns cost: N 4096, 4 rows 10.2 us at K 8192, 20.8 at K 11008; 8 rows 18.7
+  // and 31.9.
   const int64_t sets = p.offsets == nullptr ? 1 : p.E;
   if (p.offsets == nullptr ? p.R <= 2 : p.R < 2 * sets) return launch_cb<DT, 1>(p, stream);
   if (p.R < 5 * sets) return launch_cb<DT, 2>(p, stream);

@@ -119,9 +119,9 @@ def convrot_w4a16_forward(x: Tensor, qweight: Tensor, wscales: Tensor, bias, con
     linear, whose rows are the batch's samples) with the activation kept in
     ``compute_dtype`` instead of quantised to int4; ``wscales`` [N], or
     [N, K/128] for group-128 weights.  Up to 8 rows also the faster of the two
-    on the device, its rotation included (K 4096, N 24576: one row 19.7 us
-    against 33.5, 8 rows 27.1 against 32.8, 16 rows 40.7 against 32.0); called
-    from Python both take about 84 us.  The layers call
+    on the device, its rotation included (K 4096, N 24576: one row 18.9 us
+    against 33.8, 8 rows 27.1 against 32.8, 16 rows 42.0 against 32.5); called
+    from Python both take 80 to 90 us.  The layers call
     :func:`convrot_w4a4_forward`; no counterpart in the reference."""
     if x.shape[-1] != qweight.shape[-1] * 2:
         raise ValueError(f"Input K={x.shape[-1]} does not match packed qweight K={qweight.shape[-1] * 2}")
